@@ -515,6 +515,85 @@ int scgg_linear_rows_pack(const float* W, const float* b, int32_t N, int32_t K, 
 int scgg_linear_rows(const float* A, int32_t lda, const void* image, int32_t N, int32_t K, float* C, int32_t ldc,
                      const int32_t* rows, const int32_t* row_count, int32_t max_rows, int32_t relu, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Attention with positions in space.  No counterpart in the reference, whose coordinate transformer adds a position
+ * embedding to its tokens (src/bootstrap/node_coordinate_diffusion/sit_model.py:157-247) and takes one softmax map per head.
+ * These calls take fp32, bf16 and fp16 tensors [B, tokens, heads, width] with a dense last axis and any other strides (in
+ * elements); statistics, sums and angles are held in 32 bits or more and every output is rounded once.  They enqueue on
+ * `stream`, never synchronise or allocate, and may be captured into a HIP graph.  Equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------------------------- */
+#define SCGG_F32 0
+#define SCGG_BF16 1
+#define SCGG_F16 2
+
+#define SCGG_POS_F32 0
+#define SCGG_POS_F64 1
+#define SCGG_POS_I32 2
+#define SCGG_POS_I64 3
+#define SCGG_ROPE_MAX_AXES 8
+
+/* Rotary positions with several axes on the heads of q ([0]) and k ([1]); heads[1] = 0 leaves k out.  sections[a] pairs of a
+ * head turn with axis a, the j-th of them by positions[.., a] theta^(-j / sections[a]); pairs behind the last section stay.
+ * A pair is (x_2i, x_2i+1) if interleaved, else (x_i, x_{i + D/2}).  weight[0..1] (both or neither) asks for an RMS norm of
+ * every head in front of the rotation: x / sqrt(mean x^2 + eps) * weight; n_sections = 0 gives the norm alone.
+ * D: even, at most 256. */
+typedef struct scgg_rope_args {
+  const void* x[2];                    /* q, k: [B,N,heads,D] */
+  const void* g[2];                    /* backward: gradients of the outputs, same shapes */
+  void* y[2];                          /* forward: outputs; backward: gradients of q, k; contiguous */
+  const void* weight[2];               /* [D], fp32 (weight_f32) or of the tensors' type; NULL: no norm */
+  void* dweight[2];                    /* backward with weights: their gradients, of the weights' type; may be NULL */
+  const void* positions;               /* [B,N,n_sections] of pos_type, any strides; NULL if n_sections = 0 */
+  int64_t x_stride_b[2], x_stride_n[2], x_stride_h[2];
+  int64_t g_stride_b[2], g_stride_n[2], g_stride_h[2];
+  int64_t pos_stride_b, pos_stride_n, pos_stride_a;
+  double theta;
+  float eps;
+  int32_t B, N, heads[2], D;
+  int32_t dtype, weight_f32, pos_type, interleaved;
+  int32_t n_sections, sections[SCGG_ROPE_MAX_AXES];
+} scgg_rope_args;
+
+int scgg_rope_forward(const scgg_rope_args* args, void* stream);
+/* workspace: scgg_rope_workspace_bytes, 16-byte aligned, needed with weights only (NULL, 0 otherwise). */
+int scgg_rope_backward(const scgg_rope_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t scgg_rope_workspace_bytes(const scgg_rope_args* args);
+
+/* Differential attention: head h of `out` is (softmax(scale q1 k1^T) - lambda[h] softmax(scale q2 k2^T)) v, with q1, q2 the
+ * heads 2h, 2h + 1 of q, k1, k2 the heads 2g, 2g + 1 of k and v the head g of v, g = h / (H / Hkv).  key_mask[b,j] = 0 hides
+ * key j (whatever its k and v hold); causal hides key j from query i where j > i + M - N.  A query that sees no key gives a row
+ * of zeros, and no gradient.  d, dv: multiples of 8, d <= 64, dv <= 128.  Bases and strides of q, k, v and dout: multiples of
+ * 16 bytes. */
+typedef struct scgg_diff_attention_args {
+  const void* q;                       /* [B,N,2 H,d] */
+  const void* k;                       /* [B,M,2 Hkv,d] */
+  const void* v;                       /* [B,M,Hkv,dv] */
+  const float* lambda;                 /* [H] */
+  const uint8_t* key_mask;             /* [B,M], dense along M; NULL: every key is seen */
+  void* out;                           /* [B,N,H,dv] contiguous */
+  float* stats;                        /* [B,H,2,N,2]: of each map and query the largest score (in units of the base-2
+                                          exponent) and 1 / sum; written by the forward (NULL: not wanted), read by the backward */
+  const void* dout;                    /* backward: [B,N,H,dv] */
+  void* dq;                            /* contiguous, as are the other gradients */
+  void* dk;
+  void* dv_out;
+  float* dlambda;                      /* [H] */
+  int64_t q_stride_b, q_stride_n, q_stride_h;
+  int64_t k_stride_b, k_stride_n, k_stride_h;
+  int64_t v_stride_b, v_stride_n, v_stride_h;
+  int64_t dout_stride_b, dout_stride_n, dout_stride_h;
+  int64_t mask_stride_b;
+  float scale;                         /* > 0 */
+  int32_t B, N, M, H, Hkv, d, dv;
+  int32_t dtype, causal;
+} scgg_diff_attention_args;
+
+/* workspace: 256-byte aligned, contents irrelevant; a size of 0 means that none is needed. */
+size_t scgg_diff_attention_forward_workspace_bytes(const scgg_diff_attention_args* args);
+size_t scgg_diff_attention_backward_workspace_bytes(const scgg_diff_attention_args* args);
+int scgg_diff_attention_forward(const scgg_diff_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int scgg_diff_attention_backward(const scgg_diff_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

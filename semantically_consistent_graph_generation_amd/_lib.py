@@ -57,7 +57,24 @@ class TrainPackList(C.Structure):       # scgg_train_pack_list (include/scgg.h)
                 ("transpose", C.c_int32 * 10), ("count", C.c_int32)]
 
 
+class RopeArgs(C.Structure):            # scgg_rope_args (include/scgg.h)
+    _fields_ = [(k, C.c_void_p * 2) for k in ("x", "g", "y", "weight", "dweight")] + [("positions", C.c_void_p)] + \
+               [(f"{t}_stride_{a}", C.c_int64 * 2) for t in "xg" for a in "bnh"] + [(f"pos_stride_{a}", C.c_int64) for a in "bna"] + \
+               [("theta", C.c_double), ("eps", C.c_float), ("B", C.c_int32), ("N", C.c_int32), ("heads", C.c_int32 * 2)] + \
+               [(k, C.c_int32) for k in ("D", "dtype", "weight_f32", "pos_type", "interleaved", "n_sections")] + [("sections", C.c_int32 * 8)]
+
+
+class DiffAttentionArgs(C.Structure):   # scgg_diff_attention_args (include/scgg.h)
+    _fields_ = [(k, C.c_void_p) for k in ("q", "k", "v", "lambda", "key_mask", "out", "stats", "dout", "dq", "dk", "dv_out", "dlambda")] + \
+               [(f"{t}_stride_{a}", C.c_int64) for t in ("q", "k", "v", "dout") for a in "bnh"] + \
+               [("mask_stride_b", C.c_int64), ("scale", C.c_float)] + \
+               [(k, C.c_int32) for k in ("B", "N", "M", "H", "Hkv", "d", "dv", "dtype", "causal")]
+
+
 SIGNATURES = {
+    "scgg_rope_forward": (C.c_int, [C.POINTER(RopeArgs), _vp]),
+    "scgg_rope_backward": (C.c_int, [C.POINTER(RopeArgs), _vp, _sz, _vp]),
+    "scgg_rope_workspace_bytes": (_sz, [C.POINTER(RopeArgs)]),
     "scgg_train_edge_pack": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp]),
     "scgg_train_edge_forward": (C.c_int, [C.POINTER(TrainEdgeArgs), _vp]),
     "scgg_train_edge_backward": (C.c_int, [C.POINTER(TrainEdgeArgs), _vp]),

@@ -1,0 +1,449 @@
+// Rotary positions with several axes on the heads of q and k, and the RMS norm of every head in the same pass (gfx950).
+//
+// Pair i of a head belongs to the axis whose section holds i; with n_a pairs on axis a its j-th pair turns by
+// t = p_a theta^(-j / n_a).  Pairs behind the last section are left as they are.  A pair is (x_2i, x_2i+1) when interleaved,
+// else (x_i, x_{i + D/2}):  (x, y) -> (x cos t - y sin t, x sin t + y cos t); the backward turns by -t.
+// With weights, n = h w with h = x / sqrt(mean x^2 + eps) is rotated instead of x, and backward
+//   u = R^T g,  dw = sum over tokens and heads of u h,  dx = (u w - h mean(u w h)) / sqrt(mean x^2 + eps).
+//
+// Bound: HBM (x in, y out; backward g, x in, dx out).  A workgroup takes a tile of tokens.  Its threads first form the cosines
+// and sines of the tile, each once for all heads of q and k: positions reach 1e6 and beyond, so the angle is a product in
+// 64 bits, reduced to an eighth of a turn there, and only then rounded to 32.  Then the heads stream through, 16 B per load: a
+// head belongs to a power of two of lanes that hold whole pairs, so the rotation needs no exchange and the norm one butterfly.
+// Statistics and products are 32-bit, each output is rounded once.  The weight gradients are summed per lane (a lane keeps
+// its channels), per workgroup through LDS, and over the workgroups by a second kernel in a fixed order: no atomics, equal
+// calls give equal bits.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/scgg.h"
+#include "kernels.h"
+
+namespace scgg {
+namespace {
+
+constexpr int ROPE_MAX_PAIRS = 128;      // head width up to 256
+constexpr int ROPE_TILE = 16;            // tokens per workgroup tile at most
+constexpr int ROPE_TRAIN_GROUPS = 1024;  // workgroups of a backward with weights: rows of the partial sums
+
+struct RopeArgs {
+  const void* x[2];            // q, k as the forward takes them (backward with weights: again; without: unused)
+  const void* g[2];            // backward: gradients of the outputs
+  void* y[2];                  // forward: outputs; backward: gradients of q, k.  [B,N,heads,D] contiguous
+  const void* w[2];            // norm weights [D] or null
+  long long xb[2], xn[2], xh[2], gb[2], gn[2], gh[2];
+  const void* pos;
+  long long pb, pn, pa;
+  float* partial;              // [gridDim.x][2][D]
+  int heads[2];
+  int N, D, pairs, tile, pos_type, w_f32, interleaved, lanes;
+  int flat;                    // every batch stride is N token strides: the token's number is its place
+  unsigned tokens;
+  float eps;
+  double turn[ROPE_MAX_PAIRS]; // theta^(-j / n_a) / (2 pi)
+  uint8_t axis[ROPE_MAX_PAIRS];
+};
+
+template <class T, int V>
+struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
+template <class T>
+struct Vec<T, 1> { struct type { T v; __device__ T& operator[](int) { return v; } __device__ T operator[](int) const { return v; } }; };
+
+__device__ __forceinline__ void rope_place(const RopeArgs& a, unsigned tok, long long& b, long long& n) {
+  const unsigned bb = a.flat ? 0u : tok / (unsigned)a.N;
+  b = bb;
+  n = tok - bb * (unsigned)a.N;
+}
+
+__device__ __forceinline__ double rope_position(const RopeArgs& a, unsigned tok, int ax) {
+  long long b, n;
+  rope_place(a, tok, b, n);
+  const long long at = b * a.pb + n * a.pn + ax * a.pa;
+  if (a.pos_type == SCGG_POS_F32) return (double)static_cast<const float*>(a.pos)[at];
+  if (a.pos_type == SCGG_POS_F64) return static_cast<const double*>(a.pos)[at];
+  if (a.pos_type == SCGG_POS_I32) return (double)static_cast<const int32_t*>(a.pos)[at];
+  return (double)static_cast<const int64_t*>(a.pos)[at];
+}
+
+// cos and sin of `turns` whole turns: the nearest quarter turn comes off in 64 bits, so the rounding to 32 happens to an angle of at
+// most an eighth of a turn (2^-28 of a turn), and the quarter is a swap
+__device__ __forceinline__ float2 rope_cos_sin(double turns) {
+  const double q = rint(4.0 * turns);
+  const float f = (float)(turns - 0.25 * q);
+  float s, c;
+  sincospif(2.0f * f, &s, &c);
+  const int k = (int)(q - 4.0 * floor(0.25 * q));     // 0..3 (NaN and infinite positions: f and so c, s are NaN)
+  const float cs = (k & 1) ? s : c, sn = (k & 1) ? c : s;
+  return make_float2((k == 1 || k == 2) ? -cs : cs, (k & 2) ? -sn : sn);
+}
+
+template <class T>
+__device__ __forceinline__ float rope_weight(const void* w, bool f32, int i) {
+  return f32 ? static_cast<const float*>(w)[i] : (float)static_cast<const T*>(w)[i];
+}
+
+// NORM: heads are normalised first.  BWD: gradient pass.  V: elements per load, CH: pair chunks of V per lane.
+template <class T, int V, int CH, bool NORM, bool BWD>
+__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+  typedef typename Vec<T, V>::type vec;
+  extern __shared__ __align__(16) char rope_lds[];
+  float2* cs = reinterpret_cast<float2*>(rope_lds);                       // [tile][D/2]
+  const int tid = threadIdx.x, L = a.lanes, half = a.D >> 1;
+  const int chunks = half / V, group = tid / L, groups = 256 / L, lane = tid - group * L;
+  const int heads = a.heads[0] + a.heads[1];
+  int c0[CH], c1[CH];                                                     // element offsets of the lane's pairs: (c0 + i, c1 + i) or neighbours
+  bool on[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int ch = lane + c * L;
+    on[c] = ch < chunks;
+    c0[c] = a.interleaved ? 2 * V * ch : V * ch;
+    c1[c] = a.interleaved ? c0[c] + V : c0[c] + half;
+  }
+  float w[2][CH][2 * V], dw[2][CH][2 * V];
+  if (NORM) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const bool have = on[c] && a.heads[s] > 0;
+          w[s][c][i] = have ? rope_weight<T>(a.w[s], a.w_f32, c0[c] + i) : 0.f;
+          w[s][c][V + i] = have ? rope_weight<T>(a.w[s], a.w_f32, c1[c] + i) : 0.f;
+          if (BWD) dw[s][c][i] = dw[s][c][V + i] = 0.f;
+        }
+  }
+  const float inv_d = 1.0f / (float)a.D;
+  const int dk = groups / heads, dh = groups - dk * heads, k_first = group / heads, h_first = group - k_first * heads;
+  const unsigned tiles = (a.tokens + a.tile - 1) / a.tile;
+  for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const unsigned tok0 = t * a.tile;
+    const int count = (int)min(a.tokens - tok0, (unsigned)a.tile);
+    if (a.pairs > 0) {
+      __syncthreads();                                                    // the previous tile's readers are done
+      for (int i = tid; i < count * half; i += 256) {
+        const int k = i / half, p = i - k * half;
+        float2 v = make_float2(1.f, 0.f);
+        if (p < a.pairs) {
+          v = rope_cos_sin(rope_position(a, tok0 + k, a.axis[p]) * a.turn[p]);
+        }
+        cs[i] = v;
+      }
+      __syncthreads();
+    }
+    int k = k_first, h = h_first;                                         // token of the tile, head among q's and k's
+    while (k < count) {                                                   // uniform over the L lanes of a head
+      const bool s = h >= a.heads[0];                                     // a head of k
+      const int hh = s ? h - a.heads[0] : h;
+      const unsigned tok = tok0 + k;
+      long long b, n;
+      rope_place(a, tok, b, n);
+      const T* xp = (BWD && !NORM) ? nullptr
+                                   : static_cast<const T*>(s ? a.x[1] : a.x[0]) + b * (s ? a.xb[1] : a.xb[0]) +
+                                         n * (s ? a.xn[1] : a.xn[0]) + hh * (s ? a.xh[1] : a.xh[0]);
+      const T* gp = BWD ? static_cast<const T*>(s ? a.g[1] : a.g[0]) + b * (s ? a.gb[1] : a.gb[0]) + n * (s ? a.gn[1] : a.gn[0]) +
+                              hh * (s ? a.gh[1] : a.gh[0])
+                        : nullptr;
+      T* yp = static_cast<T*>(s ? a.y[1] : a.y[0]) + ((long long)tok * (s ? a.heads[1] : a.heads[0]) + hh) * a.D;
+      float x[CH][2 * V], g[CH][2 * V];
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (on[c]) {
+          if (!BWD || NORM) {
+            const vec v0 = *reinterpret_cast<const vec*>(xp + c0[c]), v1 = *reinterpret_cast<const vec*>(xp + c1[c]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { x[c][i] = (float)v0[i]; x[c][V + i] = (float)v1[i]; }
+          }
+          if (BWD) {
+            const vec v0 = *reinterpret_cast<const vec*>(gp + c0[c]), v1 = *reinterpret_cast<const vec*>(gp + c1[c]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { g[c][i] = (float)v0[i]; g[c][V + i] = (float)v1[i]; }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) x[c][i] = g[c][i] = 0.f;
+        }
+        if (NORM) {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) ss = fmaf(x[c][i], x[c][i], ss);
+        }
+      }
+      float r = 1.f;
+      if (NORM) {
+        for (int m = 1; m < L; m <<= 1) ss += __shfl_xor(ss, m);
+        r = rsqrtf(ss * inv_d + a.eps);
+      }
+      float dot = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (!on[c]) continue;
+        float2 t2[V];
+        const int p0 = V * (lane + c * L);
+        if (a.pairs > 0) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) t2[i] = cs[k * half + p0 + i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) t2[i] = make_float2(1.f, 0.f);
+        }
+        float* z = BWD ? g[c] : x[c];
+        if (NORM && !BWD) {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) z[i] = z[i] * r * (s ? w[1][c][i] : w[0][c][i]);
+        }
+        if (a.interleaved) {
+          // elements e = 0 .. 2V-1 of the lane are neighbours: pair i is (2i, 2i + 1)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float p = z[2 * i], q = z[2 * i + 1], sn = BWD ? -t2[i].y : t2[i].y;
+            z[2 * i] = fmaf(p, t2[i].x, -(q * sn));
+            z[2 * i + 1] = fmaf(p, sn, q * t2[i].x);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float p = z[i], q = z[V + i], sn = BWD ? -t2[i].y : t2[i].y;
+            z[i] = fmaf(p, t2[i].x, -(q * sn));
+            z[V + i] = fmaf(p, sn, q * t2[i].x);
+          }
+        }
+        if (NORM && BWD) {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) {
+            const float hx = x[c][i] * r;
+            const float du = z[i] * hx, ws = s ? w[1][c][i] : w[0][c][i];
+            dw[0][c][i] += s ? 0.f : du;
+            dw[1][c][i] += s ? du : 0.f;
+            dot = fmaf(du, ws, dot);
+            x[c][i] = hx;
+            z[i] *= ws;
+          }
+        }
+      }
+      if (NORM && BWD) {
+        for (int m = 1; m < L; m <<= 1) dot += __shfl_xor(dot, m);
+        dot *= inv_d;
+      }
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (!on[c]) continue;
+        vec v0, v1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float p = BWD ? g[c][i] : x[c][i], q = BWD ? g[c][V + i] : x[c][V + i];
+          if (NORM && BWD) { p = r * fmaf(-x[c][i], dot, p); q = r * fmaf(-x[c][V + i], dot, q); }
+          v0[i] = (T)p;
+          v1[i] = (T)q;
+        }
+        *reinterpret_cast<vec*>(yp + c0[c]) = v0;
+        *reinterpret_cast<vec*>(yp + c1[c]) = v1;
+      }
+      h += dh;
+      k += dk;
+      if (h >= heads) { h -= heads; ++k; }
+    }
+  }
+  if (NORM && BWD) {
+    // the workgroup's sums: [groups][D] of LDS per side, groups added in order
+    float* red = reinterpret_cast<float*>(rope_lds);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (on[c]) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) { red[group * a.D + c0[c] + i] = dw[s][c][i]; red[group * a.D + c1[c] + i] = dw[s][c][V + i]; }
+        }
+      __syncthreads();
+      for (int d = tid; d < a.D; d += 256) {
+        float v = 0.f;
+        for (int q = 0; q < groups; ++q) v += red[q * a.D + d];
+        a.partial[((long long)blockIdx.x * 2 + s) * a.D + d] = v;
+      }
+    }
+  }
+}
+
+// out[s][d] = sum of the workgroups' partials: 16 columns x 16 row lanes per workgroup, lanes added in order
+template <class T>
+__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ partial, int rows, int D, int w_f32, void* dw0, void* dw1) {
+  __shared__ float red[16][17];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), rl = threadIdx.x >> 4;
+  float v = 0.f;
+  if (c < 2 * D)
+    for (int r = rl; r < rows; r += 16) v += partial[(long long)r * 2 * D + c];
+  red[rl][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (rl != 0 || c >= 2 * D) return;
+  for (int q = 1; q < 16; ++q) v += red[q][threadIdx.x & 15];
+  void* o = c < D ? dw0 : dw1;
+  if (o == nullptr) return;
+  const int d = c < D ? c : c - D;
+  if (w_f32) static_cast<float*>(o)[d] = v;
+  else static_cast<T*>(o)[d] = (T)v;
+}
+
+template <class T, int V, int CH, bool NORM>
+void rope_launch2(const RopeArgs& a, bool bwd, unsigned blocks, size_t lds, hipStream_t st) {
+  if (bwd) hipLaunchKernelGGL((rope_kernel<T, V, CH, NORM, true>), dim3(blocks), dim3(256), lds, st, a);
+  else hipLaunchKernelGGL((rope_kernel<T, V, CH, NORM, false>), dim3(blocks), dim3(256), lds, st, a);
+}
+template <class T, int V, int CH>
+void rope_launch1(const RopeArgs& a, bool norm, bool bwd, unsigned blocks, size_t lds, hipStream_t st) {
+  if (norm) rope_launch2<T, V, CH, true>(a, bwd, blocks, lds, st);
+  else rope_launch2<T, V, CH, false>(a, bwd, blocks, lds, st);
+}
+template <class T>
+void rope_launch(const RopeArgs& a, int vec, bool norm, bool bwd, unsigned blocks, size_t lds, hipStream_t st) {
+  constexpr int W = 16 / sizeof(T);
+  if (vec == W) rope_launch1<T, W, 1>(a, norm, bwd, blocks, lds, st);
+  else if (vec == 2) rope_launch1<T, 2, 1>(a, norm, bwd, blocks, lds, st);
+  else rope_launch1<T, 1, 2>(a, norm, bwd, blocks, lds, st);
+}
+
+int rope_lanes(int chunks) {
+  int L = 1;
+  while (L < chunks && L < 64) L <<= 1;
+  return L;
+}
+
+// The plan of a call: elements per load, lanes per head, tokens per tile, workgroups.
+struct RopePlan { int vec, lanes, tile; long long blocks; size_t lds; };
+void rope_plan(const scgg_rope_args* p, bool bwd, bool norm, RopePlan* out) {
+  const int size = p->dtype == SCGG_F32 ? 4 : 2, half = p->D / 2, wide = 16 / size;
+  auto fits = [&](int v) {   // every row of every head starts at a multiple of the load's width
+    if (half % v != 0) return false;
+    const long long by = (long long)v * size;
+    for (int s = 0; s < 2; ++s) {
+      if (p->heads[s] == 0) continue;
+      uintptr_t all = reinterpret_cast<uintptr_t>(p->y[s]);
+      if (!bwd || norm) all |= reinterpret_cast<uintptr_t>(p->x[s]) | (uintptr_t)((p->x_stride_b[s] | p->x_stride_n[s] | p->x_stride_h[s]) * size);
+      if (bwd) all |= reinterpret_cast<uintptr_t>(p->g[s]) | (uintptr_t)((p->g_stride_b[s] | p->g_stride_n[s] | p->g_stride_h[s]) * size);
+      if (all % by != 0) return false;
+    }
+    return true;
+  };
+  out->vec = fits(wide) ? wide : fits(2) ? 2 : 1;
+  out->lanes = rope_lanes(half / out->vec);
+  const long long tokens = (long long)p->B * p->N;
+  // long inputs: 16 tokens share a tile's set-up; short ones: one token each, over as many workgroups as there are
+  long long tile = tokens / 1024;
+  out->tile = (int)(tile < 1 ? 1 : tile > ROPE_TILE ? ROPE_TILE : tile);
+  const long long tiles = (tokens + out->tile - 1) / out->tile;
+  const long long cap = bwd && norm ? ROPE_TRAIN_GROUPS : tiles;
+  out->blocks = tiles < cap ? tiles : cap;
+  out->lds = p->n_sections > 0 ? (size_t)out->tile * half * sizeof(float2) : 0;
+  if (bwd && norm) {
+    const size_t red = (size_t)(256 / out->lanes) * p->D * sizeof(float);
+    if (red > out->lds) out->lds = red;
+  }
+}
+
+int rope_check(const scgg_rope_args* p, const char* what) {
+  if (!p) return fail("%s: null argument", what);
+  if (p->dtype != SCGG_F32 && p->dtype != SCGG_BF16 && p->dtype != SCGG_F16) return fail("%s: unknown dtype %d", what, p->dtype);
+  if (p->B < 0 || p->N < 0 || p->heads[0] < 0 || p->heads[1] < 0 || p->D < 2) return fail("%s: bad shape", what);
+  if (p->D % 2 != 0 || p->D > 2 * ROPE_MAX_PAIRS) return fail("%s: head width %d: even and at most %d is supported", what, p->D, 2 * ROPE_MAX_PAIRS);
+  if (p->heads[0] > 65535 || p->heads[1] > 65535) return fail("%s: too many heads", what);
+  if (p->n_sections < 0 || p->n_sections > SCGG_ROPE_MAX_AXES) return fail("%s: %d axes: at most %d are supported", what, p->n_sections, SCGG_ROPE_MAX_AXES);
+  long long pairs = 0;
+  for (int i = 0; i < p->n_sections; ++i) {
+    if (p->sections[i] < 0) return fail("%s: a section has %d pairs", what, p->sections[i]);
+    pairs += p->sections[i];
+  }
+  if (pairs > p->D / 2) return fail("%s: the sections take %lld pairs, a head of width %d has %d", what, pairs, p->D, p->D / 2);
+  if (p->n_sections > 0) {
+    if (!(p->theta > 0.0) || !isfinite(p->theta)) return fail("%s: theta has to be positive and finite", what);
+    if (!p->positions && (long long)p->B * p->N > 0) return fail("%s: sections without positions", what);
+    if (p->pos_type < SCGG_POS_F32 || p->pos_type > SCGG_POS_I64) return fail("%s: unknown position type", what);
+  }
+  if ((long long)p->B * p->N > 0x7fffffffLL - 256) return fail("%s: too many tokens for one launch", what);
+  const bool norm = p->weight[0] || p->weight[1];
+  for (int s = 0; s < 2; ++s) {
+    if (p->heads[s] == 0 || p->B == 0 || p->N == 0) continue;
+    if (norm && !p->weight[s]) return fail("%s: a norm needs the weights of q and of k", what);
+    if (!p->y[s]) return fail("%s: null output", what);
+  }
+  if (norm && !(p->eps >= 0.f)) return fail("%s: eps has to be at least 0", what);
+  return 0;
+}
+
+int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  const bool norm = p->weight[0] || p->weight[1];
+  for (int s = 0; s < 2 && (long long)p->B * p->N > 0; ++s) {
+    if (p->heads[s] == 0) continue;
+    if ((!bwd || norm) && !p->x[s]) return fail("%s: null input", what);
+    if (bwd && !p->g[s]) return fail("%s: null gradient", what);
+  }
+  RopePlan plan;
+  rope_plan(p, bwd, norm, &plan);
+  if ((long long)p->heads[0] + p->heads[1] == 0) plan.blocks = 0;
+  RopeArgs a = {};
+  for (int s = 0; s < 2; ++s) {
+    a.x[s] = p->x[s]; a.g[s] = p->g[s]; a.y[s] = p->y[s]; a.w[s] = p->weight[s]; a.heads[s] = p->heads[s];
+    a.xb[s] = p->x_stride_b[s]; a.xn[s] = p->x_stride_n[s]; a.xh[s] = p->x_stride_h[s];
+    a.gb[s] = p->g_stride_b[s]; a.gn[s] = p->g_stride_n[s]; a.gh[s] = p->g_stride_h[s];
+  }
+  a.pos = p->positions; a.pb = p->pos_stride_b; a.pn = p->pos_stride_n; a.pa = p->pos_stride_a; a.pos_type = p->pos_type;
+  a.N = p->N > 0 ? p->N : 1; a.D = p->D; a.tile = plan.tile; a.w_f32 = p->weight_f32; a.interleaved = p->interleaved != 0;
+  a.lanes = plan.lanes; a.tokens = (unsigned)(p->B * p->N); a.eps = p->eps;
+  a.flat = 1;
+  for (int s = 0; s < 2; ++s) {
+    if (p->heads[s] == 0 || p->B <= 1) continue;
+    if (!bwd || norm) a.flat &= p->x_stride_b[s] == p->x_stride_n[s] * p->N;
+    if (bwd) a.flat &= p->g_stride_b[s] == p->g_stride_n[s] * p->N;
+  }
+  if (p->B > 1 && p->n_sections > 0) a.flat &= p->pos_stride_b == p->pos_stride_n * p->N;
+  for (int i = 0; i < p->n_sections; ++i)
+    for (int j = 0; j < p->sections[i]; ++j) {
+      a.turn[a.pairs] = pow(p->theta, -(double)j / (double)p->sections[i]) * 0.15915494309189533577;   // 1 / (2 pi)
+      a.axis[a.pairs++] = (uint8_t)i;
+    }
+  if (a.pairs == 0 && !(bwd && norm)) plan.lds = 0;
+  if (bwd && norm) {
+    const size_t need = (size_t)plan.blocks * 2 * p->D * sizeof(float);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
+    a.partial = static_cast<float*>(workspace);
+  }
+  if (plan.blocks > 0) {
+    if (p->dtype == SCGG_F32) rope_launch<float>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
+    else if (p->dtype == SCGG_BF16) rope_launch<__bf16>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
+    else rope_launch<_Float16>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
+  }
+  if (bwd && norm && (p->dweight[0] || p->dweight[1])) {
+    const dim3 grid((unsigned)((2 * p->D + 15) / 16));
+    const int rows = (int)plan.blocks;   // none: the sums are zero
+    if (p->dtype == SCGG_F32) hipLaunchKernelGGL(rope_dw_kernel<float>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    else if (p->dtype == SCGG_BF16) hipLaunchKernelGGL(rope_dw_kernel<__bf16>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    else hipLaunchKernelGGL(rope_dw_kernel<_Float16>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace scgg
+
+using namespace scgg;
+
+extern "C" size_t scgg_rope_workspace_bytes(const scgg_rope_args* p) {
+  if (rope_check(p, "rope_workspace_bytes")) return 0;
+  return (size_t)ROPE_TRAIN_GROUPS * 2 * p->D * sizeof(float);
+}
+
+extern "C" int scgg_rope_forward(const scgg_rope_args* p, void* stream) {
+  if (rope_check(p, "rope_forward")) return -1;
+  return rope_run(p, false, "rope_forward", nullptr, 0, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int scgg_rope_backward(const scgg_rope_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (rope_check(p, "rope_backward")) return -1;
+  return rope_run(p, true, "rope_backward", workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
