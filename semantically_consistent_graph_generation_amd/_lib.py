@@ -75,6 +75,10 @@ SIGNATURES = {
     "scgg_rope_forward": (C.c_int, [C.POINTER(RopeArgs), _vp]),
     "scgg_rope_backward": (C.c_int, [C.POINTER(RopeArgs), _vp, _sz, _vp]),
     "scgg_rope_workspace_bytes": (_sz, [C.POINTER(RopeArgs)]),
+    "scgg_diff_attention_forward": (C.c_int, [C.POINTER(DiffAttentionArgs), _vp, _sz, _vp]),
+    "scgg_diff_attention_backward": (C.c_int, [C.POINTER(DiffAttentionArgs), _vp, _sz, _vp]),
+    "scgg_diff_attention_forward_workspace_bytes": (_sz, [C.POINTER(DiffAttentionArgs)]),
+    "scgg_diff_attention_backward_workspace_bytes": (_sz, [C.POINTER(DiffAttentionArgs)]),
     "scgg_train_edge_pack": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp]),
     "scgg_train_edge_forward": (C.c_int, [C.POINTER(TrainEdgeArgs), _vp]),
     "scgg_train_edge_backward": (C.c_int, [C.POINTER(TrainEdgeArgs), _vp]),

@@ -1,0 +1,353 @@
+// Differential attention (gfx950): shared parts of the forward and backward kernels.
+//
+//   out_h = A v,  A = P1 - lambda_h P2,  P_i = softmax(scale q_i k_i^T)
+//
+// Everything runs on v_mfma_f32_32x32x16: lane l supplies row / column l & 31 and the 8 contraction slots of half l >> 5; the
+// result has column l & 31 and rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).  A product whose result feeds the next one is
+// formed with the axis that the next one sums over in the rows: the 16 values that a lane then holds are the operand of two
+// products over 16 slots each (the slots' order is the rows' order, so the other operand is read in that order).
+//
+// Types: bf16 and fp16 multiply as they are.  fp32 is split exactly into three bf16 terms (h + m + l) and a product is the six
+// leading partial products, which keeps fp32's accuracy at 2.7 times the rate of the fp32 matrix instructions.  A tile in LDS has a plane per
+// term, so the kernels are the same for all types.
+//
+// Tiles in LDS: 64 rows (keys, or queries in the dK / dV kernel) of 64 m bytes, with the 16-byte chunks of a row permuted by
+// the row: the row-wise reads (b128: 16 rows at one chunk) and the transposing ones (tr_b64: 4 rows at 32 columns) then both meet
+// every bank once.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/scgg.h"
+#include "kernels.h"
+
+namespace scgg {
+namespace diffattn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned long long u64;
+
+constexpr int TILE = 64;          // keys (or queries) per tile: one bit each in a wave-wide ballot
+constexpr int THREADS = 256;
+
+struct Args {
+  const void *q, *k, *v, *dout;
+  const float* lambda;
+  const uint8_t* mask;
+  void *out, *dq, *dk, *dv;
+  float2* stats;                  // [B,H,2,N]: scale log2(e) max, 1 / sum
+  float* delta;                   // [B,H,2,N]: sum_j P_i dP
+  float* part;                    // split forward: partial results (split_kernel)
+  long long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh, mb;
+  float scale, c;                 // c = scale log2(e)
+  int B, N, M, H, Hkv, d, dv_w, causal;
+  int splits, split_tiles;        // split forward: workgroups along the keys and the tiles each of them takes
+};
+
+// ------------------------------------------------------------------------------------------------ element types
+template <int P>
+struct Frag { u32x4 p[P]; };      // 8 contraction slots of a lane, P planes
+
+template <class T>
+struct Type;
+template <>
+struct Type<__bf16> {
+  static constexpr int planes = 1;
+  static __device__ __forceinline__ f32x16 mma1(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Type<_Float16> {
+  static constexpr int planes = 1;
+  static __device__ __forceinline__ f32x16 mma1(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Type<float> {
+  static constexpr int planes = 3;
+  static __device__ __forceinline__ f32x16 mma1(u32x4 a, u32x4 b, f32x16 c) { return Type<__bf16>::mma1(a, b, c); }
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// A sum of products over the operands' slots, as a matrix instruction rounds it: fp32's six partial products in one accumulator would be
+// six roundings (with a bias of some 1e-3 of a step) of a sum that grows, so the five small ones have an accumulator of their own.
+template <class T>
+struct Dot {
+  f32x16 a = zero16(), small = zero16();
+  __device__ __forceinline__ void add(const Frag<Type<T>::planes>& x, const Frag<Type<T>::planes>& y) {
+    if constexpr (Type<T>::planes == 1) {
+      a = Type<T>::mma1(x.p[0], y.p[0], a);
+    } else {
+      small = Type<T>::mma1(x.p[2], y.p[0], small);
+      small = Type<T>::mma1(x.p[0], y.p[2], small);
+      small = Type<T>::mma1(x.p[1], y.p[1], small);
+      small = Type<T>::mma1(x.p[1], y.p[0], small);
+      small = Type<T>::mma1(x.p[0], y.p[1], small);
+      a = Type<T>::mma1(x.p[0], y.p[0], a);
+    }
+  }
+  __device__ __forceinline__ f32x16 sum() const {
+    if constexpr (Type<T>::planes == 1) return a;
+    else return a + small;
+  }
+};
+
+// o += x y, for sums over many tiles: fp32's six products are added up from zero and rounded into the long sum once
+template <class T>
+__device__ __forceinline__ void accumulate(f32x16& o, const Frag<Type<T>::planes>& x, const Frag<Type<T>::planes>& y) {
+  if constexpr (Type<T>::planes == 1) {
+    o = Type<T>::mma1(x.p[0], y.p[0], o);
+  } else {
+    f32x16 t = Type<T>::mma1(x.p[2], y.p[0], zero16());       // smallest first
+    t = Type<T>::mma1(x.p[0], y.p[2], t);
+    t = Type<T>::mma1(x.p[1], y.p[1], t);
+    t = Type<T>::mma1(x.p[1], y.p[0], t);
+    t = Type<T>::mma1(x.p[0], y.p[1], t);
+    t = Type<T>::mma1(x.p[0], y.p[0], t);
+    o += t;
+  }
+}
+
+// two fp32 values into one packed word of each plane
+template <class T>
+__device__ __forceinline__ void pack2(float x, float y, unsigned (&out)[Type<T>::planes]) {
+  if constexpr (Type<T>::planes == 1) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    t2 v;
+    v[0] = (T)x;
+    v[1] = (T)y;
+    out[0] = __builtin_bit_cast(unsigned, v);
+  } else {                         // x = h + m + l by truncation: exact
+    unsigned u = __float_as_uint(x), w = __float_as_uint(y);
+    out[0] = __builtin_amdgcn_perm(w, u, 0x07060302u);
+    x -= __uint_as_float(u & 0xffff0000u);
+    y -= __uint_as_float(w & 0xffff0000u);
+    u = __float_as_uint(x);
+    w = __float_as_uint(y);
+    out[1] = __builtin_amdgcn_perm(w, u, 0x07060302u);
+    x -= __uint_as_float(u & 0xffff0000u);
+    y -= __uint_as_float(w & 0xffff0000u);
+    out[2] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ Frag<Type<T>::planes> pack8(const float* x) {
+  Frag<Type<T>::planes> f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned w[Type<T>::planes];
+    pack2<T>(x[2 * i], x[2 * i + 1], w);
+#pragma unroll
+    for (int p = 0; p < Type<T>::planes; ++p) f.p[p][i] = w[p];
+  }
+  return f;
+}
+
+// 8 elements as they lie in memory
+template <class T>
+struct Raw {
+  u32x4 a;
+  __device__ __forceinline__ void load(const T* p) { a = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void clear() { a = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ Frag<1> frag() const { return Frag<1>{{a}}; }
+};
+template <>
+struct Raw<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const f32x4*>(p); b = *reinterpret_cast<const f32x4*>(p + 4); }
+  __device__ __forceinline__ void clear() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ Frag<3> frag() const {
+    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return pack8<float>(x);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ tiles in LDS
+// A tile of `ROWS` rows and W columns, P planes; row = 2 W bytes (a multiple of 64)
+template <int W, int P, int ROWS = TILE>
+struct Tile {
+  static constexpr int ROW = 2 * W, PLANE = ROWS * ROW, BYTES = P * PLANE;
+  static_assert(ROW % 64 == 0, "rows of whole 64-byte groups");
+  static __device__ __forceinline__ int place(int row, int chunk) {    // byte offset of a row's 16-byte chunk
+    int c;
+    if constexpr (ROW % 256 == 0) c = chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
+    else if constexpr (ROW % 128 == 0) c = chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+    else c = chunk ^ ((row >> 2) & 3);
+    return row * ROW + c * 16;
+  }
+  static __device__ __forceinline__ void put(char* base, int row, int chunk, const Frag<P>& f) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(base + p * PLANE + place(row, chunk)) = f.p[p];
+  }
+  // operand whose row / column index is the tile's row and whose slots are columns 8 chunk .. 8 chunk + 7
+  static __device__ __forceinline__ Frag<P> rows(const char* base, int row, int chunk) {
+    Frag<P> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const u32x4*>(base + p * PLANE + place(row, chunk));
+    return f;
+  }
+  // operand whose row / column index is the tile's column col0 + (lane & 31) and whose slots are the 16 rows from row0 in
+  // the order of a result's rows.  `last`: first column behind the ones that matter; lanes behind it read a neighbour's
+  static __device__ __forceinline__ Frag<P> cols(const char* base, int row0, int col0, int lane, int last) {
+    const int i = lane & 15, sub = (lane >> 4) & 1, g = lane >> 5;
+    int col = col0 + 16 * sub;
+    if (col >= last) col = col0;
+    col += 4 * (i & 3);
+    Frag<P> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = row0 + 8 * u + 4 * g + (i >> 2);
+        const char* at = base + p * PLANE + place(row, col >> 3) + 2 * (col & 7);
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)at));
+        f.p[p][2 * u] = w[0];
+        f.p[p][2 * u + 1] = w[1];
+      }
+    }
+    return f;
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ which keys are seen
+// Bits of the tile that starts at key 64 t: the mask's and those inside M.  The masks' words of a window of tiles are formed at
+// once, kept in LDS, and refilled by the whole workgroup when the loop leaves the window.
+constexpr int WINDOW = 128;
+
+struct KeyBits {
+  const uint8_t* mask;             // of this sequence, or null
+  u64* words;                      // LDS [WINDOW]
+  int M, first, end;               // window: tiles [first, first + WINDOW); tiles from `end` on are not asked for
+
+  __device__ __forceinline__ void fill(int t, int wave, int lane) {
+    __syncthreads();
+    for (int i = wave; i < WINDOW; i += THREADS / 64) {
+      const long long key = (long long)(t + i) * TILE + lane;
+      const bool on = t + i < end && key < M && mask[key] != 0;
+      const u64 w = __ballot(on);
+      if (lane == 0) words[i] = w;
+    }
+    first = t;
+    __syncthreads();
+  }
+  __device__ __forceinline__ u64 inside(int t) const {
+    const long long left = (long long)M - (long long)t * TILE;
+    return left >= TILE ? ~0ull : (1ull << left) - 1;
+  }
+  // the first tile from t on that has a seen key (or `end`), and its bits; the same for all waves of the workgroup
+  __device__ __forceinline__ int next(int t, u64& bits, int wave, int lane) {
+    bits = 0;
+    if (mask == nullptr) {
+      if (t < end) bits = inside(t);
+      return t;
+    }
+    for (; t < end; ++t) {
+      if (t >= first + WINDOW) fill(t, wave, lane);
+      const u64 w = words[t - first];
+      const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)w), hi = __builtin_amdgcn_readfirstlane((unsigned)(w >> 32));
+      bits = ((u64)hi << 32) | lo;
+      if (bits != 0) break;
+    }
+    return t;
+  }
+  __device__ __forceinline__ void start(int t, int wave, int lane) {
+    first = t;
+    if (mask != nullptr && t < end) fill(t, wave, lane);
+  }
+};
+
+// bits of a tile for a query that sees keys up to `last` of it (causal)
+__device__ __forceinline__ u64 upto(long long last) { return last >= 63 ? ~0ull : last < 0 ? 0ull : (2ull << last) - 1; }
+
+// the scores of the 32-key half `hh` whose keys are not in `bits` become -inf
+__device__ __forceinline__ void hide(f32x16& s, u64 bits, int hh, int g) {
+  const unsigned w = (unsigned)(bits >> (32 * hh)) >> (4 * g);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1u ? s[r] : -INFINITY;
+}
+
+// ------------------------------------------------------------------------------------------------ staging
+// A tile's rows into registers, 8 elements a piece, and from there into LDS: the loads of the next tile are under way while
+// this one is used.  Rows whose bit is off and columns from `width` on are zeros, whatever memory holds there.
+template <class T, int W, int HEADS, int NT = THREADS>   // HEADS heads of W / HEADS columns side by side in a row
+struct Stage {
+  static constexpr int PIECES = W / 8, PER = TILE * PIECES / NT, HW = W / HEADS;
+  static_assert(TILE * PIECES % NT == 0, "whole pieces per thread");
+  typedef Tile<W, Type<T>::planes> tile;
+  Raw<T> raw[PER];
+  __device__ __forceinline__ void load(const T* base, long long row_stride, long long head_stride, long long row0, u64 bits, int width, int tid) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = tid + j * NT, row = i / PIECES, pc = i - row * PIECES;
+      const int head = HEADS == 1 ? 0 : pc / (HW / 8), col = (pc - head * (HW / 8)) * 8;
+      if (((bits >> row) & 1) && col < width) raw[j].load(base + (row0 + row) * row_stride + head * head_stride + col);
+      else raw[j].clear();
+    }
+  }
+  __device__ __forceinline__ void put(char* lds, int tid) const {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = tid + j * NT, row = i / PIECES, pc = i - row * PIECES;
+      tile::put(lds, row, pc, raw[j].frag());
+    }
+  }
+};
+
+// 32 rows as operands in registers: lane & 31 is the row, slots 16 c + 8 g ..
+template <class T, int W>
+__device__ __forceinline__ void load_rows(Frag<Type<T>::planes> (&f)[W / 16], const T* row, bool on, int width, int g) {
+#pragma unroll
+  for (int c = 0; c < W / 16; ++c) {
+    Raw<T> r;
+    const int col = 16 * c + 8 * g;
+    if (on && col < width) r.load(row + col);
+    else r.clear();
+    f[c] = r.frag();
+  }
+}
+
+// four consecutive values of a row, rounded once
+template <class T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 v;
+  v[0] = (T)a;
+  v[1] = (T)b;
+  v[2] = (T)c;
+  v[3] = (T)d;
+  *reinterpret_cast<t4*>(p) = v;
+}
+
+// Work index -> place: consecutive workgroups go to the 8 dies in turn, so a die takes a contiguous stretch of the work (the tiles
+// of one head, whose keys then stay in that die's L2).
+__device__ __forceinline__ unsigned die_major(unsigned id, unsigned total) {
+  const unsigned per = total >> 3, rest = total & 7, die = id & 7, at = id >> 3;
+  return die * per + (die < rest ? die : rest) + at;
+}
+
+// widths that a kernel is built for; the smallest pair that holds (d, dv) is taken
+#define SCGG_DIFF_WIDTHS(X) X(32, 32) X(32, 64) X(48, 96) X(64, 64) X(64, 128)
+
+template <class T> int run_forward(const Args& a, hipStream_t st);
+template <class T> int run_split(const Args& a, hipStream_t st);
+template <class T> int run_backward(const Args& a, hipStream_t st);
+
+}  // namespace diffattn
+}  // namespace scgg

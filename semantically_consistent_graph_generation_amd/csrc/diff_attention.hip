@@ -1,0 +1,142 @@
+// Differential attention: entry points, checks, workspaces and the sum for the gradient of lambda.  The kernels are in
+// diff_attention_fwd.h and diff_attention_bwd.h, compiled per element type.
+#include "diff_attention.h"
+
+namespace scgg {
+namespace diffattn {
+namespace {
+
+constexpr int SPLIT_MIN_TILES = 4;     // keys of a split workgroup at least: 4 tiles of 64
+constexpr int SPLIT_GROUPS = 1024;     // workgroups that keep the memory busy: 4 on each of 256 CUs
+
+// dlambda[h] = - sum over sequences and queries of delta_2, in a fixed order: 256 lanes, each a stretch, then a tree
+__global__ __launch_bounds__(256) void dlambda_kernel(const float* __restrict__ delta, float* __restrict__ out, int B, int H, int N) {
+  __shared__ float red[4];
+  const int h = blockIdx.x;
+  float v = 0.f;
+  for (int b = 0; b < B; ++b) {
+    const float* d = delta + (((long long)b * H + h) * 3 + 1) * N;
+    for (int n = threadIdx.x; n < N; n += 256) v += d[n];
+  }
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) out[h] = -((red[0] + red[1]) + (red[2] + red[3]));
+}
+
+int check(const scgg_diff_attention_args* p, const char* what) {
+  if (!p) return fail("%s: null argument", what);
+  if (p->dtype != SCGG_F32 && p->dtype != SCGG_BF16 && p->dtype != SCGG_F16) return fail("%s: unknown dtype %d", what, p->dtype);
+  if (p->B < 0 || p->N < 0 || p->M < 0) return fail("%s: bad shape", what);
+  if (p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0) return fail("%s: %d heads on %d key heads", what, p->H, p->Hkv);
+  if (p->d < 8 || p->dv < 8 || p->d % 8 != 0 || p->dv % 8 != 0 || p->d > 64 || p->dv > 128)
+    return fail("%s: d = %d, dv = %d: multiples of 8 with d <= 64 and dv <= 128 are supported", what, p->d, p->dv);
+  if (!(p->scale > 0.f) || !isfinite(p->scale)) return fail("%s: scale has to be positive and finite", what);
+  if (p->N > 0x7fffffff - 256 || p->M > 0x7fffffff - 256) return fail("%s: too many tokens", what);
+  if ((long long)p->B * p->H > 0x7fffffff || (long long)p->B * p->N * p->H > 0x7fffffffLL * 32) return fail("%s: too many rows", what);
+  return 0;
+}
+
+bool aligned(const scgg_diff_attention_args* p, const void* base, int64_t sb, int64_t sn, int64_t sh) {
+  const int64_t size = p->dtype == SCGG_F32 ? 4 : 2;
+  return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)((sb | sn | sh) * size)) & 15) == 0;
+}
+
+int check_inputs(const scgg_diff_attention_args* p, const char* what) {
+  const bool queries = p->B > 0 && p->N > 0, keys = p->B > 0 && p->M > 0;
+  if ((queries && !p->q) || (keys && (!p->k || !p->v)) || !p->lambda) return fail("%s: null argument", what);
+  if ((queries && !aligned(p, p->q, p->q_stride_b, p->q_stride_n, p->q_stride_h)) ||
+      (keys && (!aligned(p, p->k, p->k_stride_b, p->k_stride_n, p->k_stride_h) || !aligned(p, p->v, p->v_stride_b, p->v_stride_n, p->v_stride_h))))
+    return fail("%s: bases and strides of q, k and v have to be multiples of 16 bytes", what);
+  return 0;
+}
+
+Args make(const scgg_diff_attention_args* p) {
+  Args a = {};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.dout = p->dout; a.lambda = p->lambda; a.mask = p->key_mask;
+  a.out = p->out; a.dq = p->dq; a.dk = p->dk; a.dv = p->dv_out; a.stats = reinterpret_cast<float2*>(p->stats);
+  a.qb = p->q_stride_b; a.qn = p->q_stride_n; a.qh = p->q_stride_h;
+  a.kb = p->k_stride_b; a.kn = p->k_stride_n; a.kh = p->k_stride_h;
+  a.vb = p->v_stride_b; a.vn = p->v_stride_n; a.vh = p->v_stride_h;
+  a.gb = p->dout_stride_b; a.gn = p->dout_stride_n; a.gh = p->dout_stride_h; a.mb = p->mask_stride_b;
+  a.scale = p->scale; a.c = p->scale * 1.44269504088896340736f;
+  a.B = p->B; a.N = p->N; a.M = p->M; a.H = p->H; a.Hkv = p->Hkv; a.d = p->d; a.dv_w = p->dv; a.causal = p->causal != 0;
+  return a;
+}
+
+// Keys split over workgroups (0: not): when the rows of a key head's group fill no more than one block of 32 and there are keys to split
+void plan_split(Args& a) {
+  const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, heads = (long long)a.B * a.Hkv;
+  a.splits = 0;
+  if (rows > 32 || tiles < 2 * SPLIT_MIN_TILES) return;
+  long long s = SPLIT_GROUPS / (heads > 0 ? heads : 1);
+  if (s > tiles / SPLIT_MIN_TILES) s = tiles / SPLIT_MIN_TILES;
+  if (s < 1) s = 1;
+  a.split_tiles = (int)((tiles + s - 1) / s);
+  a.splits = (int)((tiles + a.split_tiles - 1) / a.split_tiles);
+}
+
+size_t part_bytes(const Args& a) {
+  return a.splits == 0 ? 0 : (size_t)a.B * a.H * a.N * 2 * a.splits * (2 * a.dv_w + 4) * sizeof(float);
+}
+size_t delta_bytes(const Args& a) { return (size_t)a.B * a.H * 3 * a.N * sizeof(float); }
+
+int done(int rc, const char* what) {
+  if (rc == -3) return fail("%s: too many tokens for one launch", what);
+  if (rc != 0) return fail("%s: the kernel's shared memory could not be set up", what);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail("%s: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace diffattn
+}  // namespace scgg
+
+using namespace scgg;
+using namespace scgg::diffattn;
+
+extern "C" size_t scgg_diff_attention_forward_workspace_bytes(const scgg_diff_attention_args* p) {
+  if (check(p, "diff_attention_forward_workspace_bytes")) return 0;
+  Args a = make(p);
+  plan_split(a);
+  return part_bytes(a);
+}
+
+extern "C" size_t scgg_diff_attention_backward_workspace_bytes(const scgg_diff_attention_args* p) {
+  if (check(p, "diff_attention_backward_workspace_bytes")) return 0;
+  return delta_bytes(make(p));
+}
+
+extern "C" int scgg_diff_attention_forward(const scgg_diff_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "diff_attention_forward";
+  if (check(p, what) || check_inputs(p, what)) return -1;
+  if (p->B == 0 || p->N == 0) return 0;
+  if (!p->out) return fail("%s: null output", what);
+  Args a = make(p);
+  plan_split(a);
+  const size_t need = part_bytes(a);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
+  a.part = static_cast<float*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  if (a.splits > 0) rc = p->dtype == SCGG_F32 ? run_split<float>(a, st) : p->dtype == SCGG_BF16 ? run_split<__bf16>(a, st) : run_split<_Float16>(a, st);
+  else rc = p->dtype == SCGG_F32 ? run_forward<float>(a, st) : p->dtype == SCGG_BF16 ? run_forward<__bf16>(a, st) : run_forward<_Float16>(a, st);
+  return done(rc, what);
+}
+
+extern "C" int scgg_diff_attention_backward(const scgg_diff_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "diff_attention_backward";
+  if (check(p, what) || check_inputs(p, what)) return -1;
+  const bool queries = p->B > 0 && p->N > 0, keys = p->B > 0 && p->M > 0;
+  if ((queries && (!p->dout || !p->dq || !p->stats)) || (keys && (!p->dk || !p->dv_out)) || !p->dlambda) return fail("%s: null argument", what);
+  if (queries && !aligned(p, p->dout, p->dout_stride_b, p->dout_stride_n, p->dout_stride_h))
+    return fail("%s: base and strides of dout have to be multiples of 16 bytes", what);
+  Args a = make(p);
+  const size_t need = delta_bytes(a);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
+  a.delta = static_cast<float*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int rc = p->dtype == SCGG_F32 ? run_backward<float>(a, st) : p->dtype == SCGG_BF16 ? run_backward<__bf16>(a, st) : run_backward<_Float16>(a, st);
+  if (rc == 0) hipLaunchKernelGGL(dlambda_kernel, dim3((unsigned)p->H), dim3(256), 0, st, a.delta, p->dlambda, p->B, p->H, p->N);
+  return done(rc, what);
+}

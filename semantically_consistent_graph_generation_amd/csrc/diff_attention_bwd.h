@@ -1,0 +1,463 @@
+// Differential attention, backward kernels.  Included by the translation unit of each element type.
+//
+//   dV = A^T dO,  dP = dO V^T (the same for both maps),  dS_i = w_i P_i (dP - delta_i) with w_1 = 1, w_2 = -lambda,
+//   delta_i = sum_j P_i dP,  dQ_i = scale dS_i K_i,  dK_i = scale dS_i^T Q_i,  dlambda = - sum delta_2
+//
+// Two kernels, each of which owns what it writes (no atomics): one over queries for delta and dQ, one over keys for dK and dV.
+// delta comes from a sweep of its own, formed in 32 bits: dlambda is its sum, and dS a difference with it.
+#pragma once
+#include "diff_attention_fwd.h"
+
+namespace scgg {
+namespace diffattn {
+
+template <class T, int DP, int DVP>
+struct DqShape {
+  static constexpr int P = Type<T>::planes, ND = (DP + 31) / 32;
+  typedef Tile<2 * DP, P> KTile;
+  typedef Tile<DVP, P> VTile;
+  static constexpr int MERGE = 2 * 2 * ND * 16 * 64 * 4;
+  static constexpr int TILES = KTile::BYTES + VTile::BYTES;
+  static constexpr int WORDS = TILES > MERGE ? TILES : MERGE;
+  static constexpr int LDS = WORDS + WINDOW * 8;
+  static constexpr int MIN_BLOCKS = P == 3 ? 1 : 2;
+};
+
+// delta [B,H,3,N]: delta_1, delta_2, and the largest |dP| of the query
+template <class T, int DP, int DVP, int KW>
+__global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq_kernel(Args a) {
+  typedef DqShape<T, DP, DVP> S;
+  typedef typename S::KTile KTile;
+  typedef typename S::VTile VTile;
+  constexpr int P = S::P, QW = 4 / KW, BQ = 32 * QW, ND = S::ND;
+  extern __shared__ __align__(256) char lds[];
+  char* kt = lds;
+  char* vt = lds + KTile::BYTES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
+  const int qw = wave / KW, kw = wave - qw * KW;
+  const int q_tiles = (a.N + BQ - 1) / BQ;
+  const unsigned id = die_major(blockIdx.x, gridDim.x);
+  const int bh = id / q_tiles, qt = a.causal ? q_tiles - 1 - (int)(id - bh * q_tiles) : (int)(id - bh * q_tiles);
+  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+  const int q = qt * BQ + 32 * qw + l31;
+  const bool q_on = q < a.N;
+  const long long off = (long long)a.M - a.N;
+  const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
+  const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
+
+  Frag<P> qf[2][DP / 16], gf[DVP / 16];
+  float mc[2], il[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)q * a.qn + (2ll * h + i) * a.qh, q_on, a.d, g);
+    float2 st = make_float2(INFINITY, 0.f);
+    if (q_on) st = a.stats[((long long)bh * 2 + i) * a.N + q];
+    mc[i] = st.x;
+    il[i] = st.y;
+  }
+  load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on, a.dv_w, g);
+
+  KeyBits keys;
+  keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
+  keys.words = reinterpret_cast<u64*>(lds + S::WORDS);
+  keys.M = a.M;
+  keys.end = (a.M + TILE - 1) / TILE;
+  if (a.causal) {
+    const long long q_last = (qt + 1) * BQ < a.N ? (qt + 1) * BQ - 1 : a.N - 1, last = q_last + off;
+    const int e = last < 0 ? 0 : (int)(last / TILE) + 1;
+    if (e < keys.end) keys.end = e;
+  }
+  const long long wave_last = (long long)qt * BQ + 32 * qw + 31 + off;
+
+  Stage<T, 2 * DP, 2> ks;
+  Stage<T, DVP, 1> vs;
+  auto score = [&](int i, int hh) {
+    Dot<T> s;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+    return s.sum();
+  };
+  auto dprob = [&](int hh) {
+    Dot<T> s;
+#pragma unroll
+    for (int c = 0; c < DVP / 16; ++c) s.add(VTile::rows(vt, 32 * hh + l31, 2 * c + g), gf[c]);
+    return s.sum();
+  };
+  auto seen = [&](int t, u64 bits) { return a.causal ? bits & upto(q + off - (long long)t * TILE) : bits; };
+  auto begin = [&](int& t, u64& bits) {
+    keys.start(0, wave, lane);
+    t = keys.next(0, bits, wave, lane);
+    if (t < keys.end) {
+      ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
+      vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+    }
+  };
+  auto advance = [&](int t, u64& bits_next) {       // this tile into LDS, the next one's loads under way
+    __syncthreads();
+    ks.put(kt, tid);
+    vs.put(vt, tid);
+    __syncthreads();
+    const int tn = keys.next(t + 1, bits_next, wave, lane);
+    if (tn < keys.end) {
+      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
+      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+    }
+    return tn;
+  };
+
+  float delta[2] = {0.f, 0.f}, top = 0.f;
+  u64 bits, bits_next;
+  int t;
+  begin(t, bits);
+  while (t < keys.end) {
+    const int tn = advance(t, bits_next);
+    if (!a.causal || (long long)t * TILE <= wave_last) {
+      const u64 see = seen(t, bits);
+      const bool part = __any(see != ~0ull);
+#pragma unroll
+      for (int half = 0; half < 2 / KW; ++half) {
+        const int hh = KW == 1 ? half : kw;
+        const f32x16 dp = dprob(hh);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x16 s = score(i, hh);
+          if (part) hide(s, see, hh, g);
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
+          delta[i] = fmaf(sum, il[i], delta[i]);
+        }
+        if (__is_same(T, _Float16)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+        }
+      }
+    }
+    t = tn;
+    bits = bits_next;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) delta[i] += __shfl_xor(delta[i], 32);
+  top = fmaxf(top, __shfl_xor(top, 32));
+  if constexpr (KW == 2) {
+    float* box = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    if (g == 0) { box[(wave * 3) * 32 + l31] = delta[0]; box[(wave * 3 + 1) * 32 + l31] = delta[1]; box[(wave * 3 + 2) * 32 + l31] = top; }
+    __syncthreads();
+    const int w0 = wave & ~1;
+    delta[0] = box[(w0 * 3) * 32 + l31] + box[(w0 * 3 + 3) * 32 + l31];
+    delta[1] = box[(w0 * 3 + 1) * 32 + l31] + box[(w0 * 3 + 4) * 32 + l31];
+    top = fmaxf(box[(w0 * 3 + 2) * 32 + l31], box[(w0 * 3 + 5) * 32 + l31]);
+  }
+  const float lam = a.lambda[h];
+  if (q_on && kw == 0 && g == 0) {
+    float* dst = a.delta + (long long)bh * 3 * a.N + q;
+    dst[0] = delta[0];
+    dst[a.N] = delta[1];
+    dst[2ll * a.N] = top;
+  }
+  float up = 1.f;                                   // |dS| <= 2 max(1, |lambda|) max |dP|
+  if (__is_same(T, _Float16)) up = pow2_below(16384.f, 2.f * fmaxf(1.f, fabsf(lam)) * top);
+  const float w1 = up * il[0], w2 = -up * lam * il[1];
+
+  f32x16 o[2][ND];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < ND; ++j) o[i][j] = zero16();
+  __syncthreads();
+  begin(t, bits);
+  while (t < keys.end) {
+    const int tn = advance(t, bits_next);
+    if (!a.causal || (long long)t * TILE <= wave_last) {
+      const u64 see = seen(t, bits);
+      const bool part = __any(see != ~0ull);
+#pragma unroll
+      for (int half = 0; half < 2 / KW; ++half) {
+        const int hh = KW == 1 ? half : kw;
+        const f32x16 dp = dprob(hh);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x16 s = score(i, hh);
+          if (part) hide(s, see, hh, g);
+          float ds[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])) * (i == 0 ? w1 : w2) * (dp[r] - delta[i]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const Frag<P> df = pack8<T>(ds + 8 * u);
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+              accumulate<T>(o[i][j], KTile::cols(kt, 32 * hh + 16 * u, i * DP + 32 * j, lane, (i + 1) * DP), df);
+          }
+        }
+      }
+    }
+    t = tn;
+    bits = bits_next;
+  }
+  if constexpr (KW == 2) {
+    float* box = reinterpret_cast<float*>(lds) + (size_t)qw * 2 * ND * 16 * 64;
+    __syncthreads();
+    if (kw == 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[(i * 16 + r) * 64 + lane] = o[i / ND][i % ND][r];
+    }
+    __syncthreads();
+    if (kw == 1) return;
+#pragma unroll
+    for (int i = 0; i < 2 * ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i / ND][i % ND][r] += box[(i * 16 + r) * 64 + lane];
+  }
+  if (!q_on) return;
+  const float f = a.scale / up;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    T* dst = static_cast<T*>(a.dq) + (((long long)b * a.N + q) * 2 * a.H + 2 * h + i) * a.d;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int col = 32 * j + 2 * r + 4 * g;
+        if (col < a.d) store4<T>(dst + col, o[i][j][r] * f, o[i][j][r + 1] * f, o[i][j][r + 2] * f, o[i][j][r + 3] * f);
+      }
+  }
+}
+
+template <class T, int DP, int DVP>
+struct DkvShape {
+  static constexpr int P = Type<T>::planes, ND = (DP + 31) / 32, NV = DVP / 32;
+  typedef Tile<2 * DP, P> QTile;
+  typedef Tile<DVP, P> GTile;
+  static constexpr int TILES = QTile::BYTES + GTile::BYTES;
+  static constexpr int MERGE = 2 * (2 * ND + NV) * 16 * 64 * 4;
+  static constexpr int ROWS = TILES > MERGE ? TILES : MERGE;      // offset of the rows' statistics [6][TILE]
+  static constexpr int LDS = ROWS + 6 * TILE * 4;
+};
+
+// Over keys: a wave keeps 32 of them (k1, k2 and v as operands, dK1, dK2 and dV as sums) and the queries of all heads that share the key
+// head stream by.  4 / QW groups of 32 keys, QW waves that share a tile's queries.
+template <class T, int DP, int DVP, int QW>
+__global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
+  typedef DkvShape<T, DP, DVP> S;
+  typedef typename S::QTile QTile;
+  typedef typename S::GTile GTile;
+  constexpr int P = S::P, KG = 4 / QW, BK = 32 * KG, ND = S::ND, NV = S::NV;
+  extern __shared__ __align__(256) char lds[];
+  char* qt = lds;
+  char* gt = lds + QTile::BYTES;
+  float* rowst = reinterpret_cast<float*>(lds + S::ROWS);          // mc1, il1, mc2, il2, delta1, delta2 of the tile's queries
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
+  const int kg = wave / QW, qw = wave - kg * QW;
+  const int k_tiles = (a.M + BK - 1) / BK, group = a.H / a.Hkv;
+  const unsigned id = die_major(blockIdx.x, gridDim.x);
+  const int bk = id / k_tiles, kt = id - bk * k_tiles, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int key = kt * BK + 32 * kg + l31;
+  const bool k_in = key < a.M, k_on = k_in && (a.mask == nullptr || a.mask[b * a.mb + key] != 0);
+  const long long off = (long long)a.M - a.N;                      // causal: key j is seen by the queries >= j - off
+  Frag<P> kf[2][DP / 16], vf[DVP / 16];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    load_rows<T, DP>(kf[i], static_cast<const T*>(a.k) + b * a.kb + (long long)key * a.kn + (2ll * hk + i) * a.kh, k_on, a.d, g);
+  load_rows<T, DVP>(vf, static_cast<const T*>(a.v) + b * a.vb + (long long)key * a.vn + (long long)hk * a.vh, k_on, a.dv_w, g);
+
+  f32x16 dk[2][ND], dv[NV];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < ND; ++j) dk[i][j] = zero16();
+#pragma unroll
+  for (int j = 0; j < NV; ++j) dv[j] = zero16();
+
+  float up_a = 1.f, up_s = 1.f;                                    // fp16: one scale for all heads that are summed here
+  if constexpr (__is_same(T, _Float16)) {
+    float lam = 1.f, top = 0.f;
+    for (int i = 0; i < group; ++i) lam = fmaxf(lam, fabsf(a.lambda[hk * group + i]));
+    for (int i = 0; i < group; ++i) {
+      const float* d = a.delta + ((long long)(b * a.H + hk * group + i) * 3 + 2) * a.N;
+      for (int n = tid; n < a.N; n += THREADS) top = fmaxf(top, d[n]);
+    }
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    if (lane == 0) rowst[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(rowst[0], rowst[1]), fmaxf(rowst[2], rowst[3]));
+    up_a = pow2_below(16384.f, lam);
+    up_s = pow2_below(16384.f, 2.f * lam * top);
+  }
+
+  const int n_tiles = (a.N + TILE - 1) / TILE;
+  int t_first = 0;
+  if (a.causal) {
+    const long long q_first = (long long)kt * BK - off;
+    if (q_first > 0) t_first = q_first / TILE < n_tiles ? (int)(q_first / TILE) : n_tiles;
+  }
+  const int steps = (n_tiles - t_first) * group;
+  // a workgroup whose keys are all hidden has nothing to sum
+  const bool any = __syncthreads_or(k_on);
+  Stage<T, 2 * DP, 2> qs;
+  Stage<T, DVP, 1> gs;
+  float2 rs;
+  auto load = [&](int step) {
+    const int hg = step / (n_tiles - t_first), t = t_first + step - hg * (n_tiles - t_first), h = hk * group + hg;
+    const long long left = (long long)a.N - (long long)t * TILE;
+    const u64 bits = left >= TILE ? ~0ull : (1ull << left) - 1;
+    qs.load(static_cast<const T*>(a.q) + b * a.qb + 2ll * h * a.qh, a.qn, a.qh, (long long)t * TILE, bits, a.d, tid);
+    gs.load(static_cast<const T*>(a.dout) + b * a.gb + (long long)h * a.gh, a.gn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+    const int n = t * TILE + lane;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
+    const long long bh = (long long)b * a.H + h;
+    rs = wave < 2 ? make_float2(INFINITY, 0.f) : make_float2(0.f, 0.f);
+    if (n < a.N) {
+      if (wave < 2) rs = a.stats[(bh * 2 + wave) * a.N + n];
+      else if (wave == 2) rs = make_float2(a.delta[bh * 3 * a.N + n], a.delta[(bh * 3 + 1) * a.N + n]);
+    }
+  };
+  if (any && steps > 0) load(0);
+  for (int step = 0; any && step < steps; ++step) {
+    __syncthreads();
+    qs.put(qt, tid);
+    gs.put(gt, tid);
+    if (wave < 3) { rowst[2 * wave * TILE + lane] = rs.x; rowst[(2 * wave + 1) * TILE + lane] = rs.y; }
+    __syncthreads();
+    const int hg = step / (n_tiles - t_first), t = t_first + step - hg * (n_tiles - t_first);
+    if (step + 1 < steps) load(step + 1);
+    const float lam = a.lambda[hk * group + hg];
+#pragma unroll
+    for (int half = 0; half < 2 / QW; ++half) {
+      const int hh = QW == 1 ? half : qw;
+      const long long last_q = (long long)t * TILE + 32 * hh + 31;
+      if (a.causal && last_q + off < (long long)kt * BK + 32 * kg) continue;   // no query of these sees a key of the wave
+      auto score = [&](int i) {
+        Dot<T> s;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) s.add(QTile::rows(qt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), kf[i][c]);
+        return s.sum();
+      };
+      const f32x16 s1 = score(0), s2 = score(1);
+      Dot<T> dot;
+#pragma unroll
+      for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh + l31, 2 * c + g), vf[c]);
+      const f32x16 dp = dot.sum();
+      const bool cut = a.causal && (long long)t * TILE + 32 * hh + off < (long long)kt * BK + 32 * kg + 31;
+      float pa[16], d1[16], d2[16];
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int row = 32 * hh + 8 * r4 + 4 * g;
+        const f32x4 m1 = *reinterpret_cast<const f32x4*>(rowst + row), i1 = *reinterpret_cast<const f32x4*>(rowst + TILE + row),
+                    m2 = *reinterpret_cast<const f32x4*>(rowst + 2 * TILE + row), i2 = *reinterpret_cast<const f32x4*>(rowst + 3 * TILE + row),
+                    e1 = *reinterpret_cast<const f32x4*>(rowst + 4 * TILE + row), e2 = *reinterpret_cast<const f32x4*>(rowst + 5 * TILE + row);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = 4 * r4 + x;
+          float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -m1[x])) * i1[x];
+          float p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -m2[x])) * i2[x];
+          if (cut && key > t * (long long)TILE + row + x + off) p1 = p2 = 0.f;
+          p2 *= -lam;
+          pa[r] = (p1 + p2) * up_a;
+          d1[r] = p1 * (dp[r] - e1[x]) * up_s;
+          d2[r] = p2 * (dp[r] - e2[x]) * up_s;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row0 = 32 * hh + 16 * u;
+        const Frag<P> fa = pack8<T>(pa + 8 * u), f1 = pack8<T>(d1 + 8 * u), f2 = pack8<T>(d2 + 8 * u);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) accumulate<T>(dv[j], GTile::cols(gt, row0, 32 * j, lane, DVP), fa);
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          accumulate<T>(dk[0][j], QTile::cols(qt, row0, 32 * j, lane, DP), f1);
+          accumulate<T>(dk[1][j], QTile::cols(qt, row0, DP + 32 * j, lane, 2 * DP), f2);
+        }
+      }
+    }
+  }
+  if constexpr (QW == 2) {
+    float* box = reinterpret_cast<float*>(lds) + (size_t)kg * (2 * ND + NV) * 16 * 64;
+    __syncthreads();
+    if (qw == 1) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[(j * 16 + r) * 64 + lane] = dv[j][r];
+#pragma unroll
+      for (int j = 0; j < 2 * ND; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[((NV + j) * 16 + r) * 64 + lane] = dk[j / ND][j % ND][r];
+    }
+    __syncthreads();
+    if (qw == 1) return;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dv[j][r] += box[(j * 16 + r) * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 2 * ND; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[j / ND][j % ND][r] += box[((NV + j) * 16 + r) * 64 + lane];
+  }
+  if (!k_in) return;
+  const float fv = k_on ? 1.f / up_a : 0.f, fk = k_on ? a.scale / up_s : 0.f;
+  auto out = [&](float x, float f) { return k_on ? x * f : 0.f; };   // a hidden key's sums may hold anything
+  T* dst = static_cast<T*>(a.dv) + (((long long)b * a.M + key) * a.Hkv + hk) * a.dv_w;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int col = 32 * j + 2 * r + 4 * g;
+      if (col < a.dv_w) store4<T>(dst + col, out(dv[j][r], fv), out(dv[j][r + 1], fv), out(dv[j][r + 2], fv), out(dv[j][r + 3], fv));
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    T* kd = static_cast<T*>(a.dk) + (((long long)b * a.M + key) * 2 * a.Hkv + 2 * hk + i) * a.d;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int col = 32 * j + 2 * r + 4 * g;
+        if (col < a.d) store4<T>(kd + col, out(dk[i][j][r], fk), out(dk[i][j][r + 1], fk), out(dk[i][j][r + 2], fk), out(dk[i][j][r + 3], fk));
+      }
+  }
+}
+
+template <class T, int DP, int DVP, int KW>
+int launch_dq(const Args& a, hipStream_t st) {
+  typedef DqShape<T, DP, DVP> S;
+  static LdsAttrOnce once;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
+  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
+  if (blocks > 0x7fffffffLL) return -3;
+  if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  return 0;
+}
+
+template <class T, int DP, int DVP, int QW>
+int launch_dkv(const Args& a, hipStream_t st) {
+  typedef DkvShape<T, DP, DVP> S;
+  static LdsAttrOnce once;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, QW>), S::LDS)) return -2;
+  const long long blocks = (long long)a.B * a.Hkv * ((a.M + 128 / QW - 1) / (128 / QW));
+  if (blocks > 0x7fffffffLL) return -3;
+  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, QW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  return 0;
+}
+
+template <class T, int DP, int DVP>
+int launch_bwd(const Args& a, hipStream_t st) {
+  const bool few_q = (long long)a.B * a.H * ((a.N + 127) / 128) < 512, few_k = (long long)a.B * a.Hkv * ((a.M + 127) / 128) < 256;
+  if (const int rc = few_q ? launch_dq<T, DP, DVP, 2>(a, st) : launch_dq<T, DP, DVP, 1>(a, st)) return rc;
+  return few_k ? launch_dkv<T, DP, DVP, 2>(a, st) : launch_dkv<T, DP, DVP, 1>(a, st);
+}
+
+template <class T>
+int run_backward(const Args& a, hipStream_t st) {
+#define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return launch_bwd<T, DP, DVP>(a, st);
+  SCGG_DIFF_WIDTHS(SCGG_X)
+#undef SCGG_X
+  return -1;
+}
+
+}  // namespace diffattn
+}  // namespace scgg

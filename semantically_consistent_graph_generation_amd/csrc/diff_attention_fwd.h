@@ -1,0 +1,443 @@
+// Differential attention, forward kernels.  Included by the translation unit of each element type.
+#pragma once
+#include "diff_attention.h"
+
+namespace scgg {
+namespace diffattn {
+
+// fp16 holds values below 2^-14 with fewer bits: A and dS are multiplied by a power of two that brings their bound near 2^14
+__device__ __forceinline__ float pow2_below(float limit, float bound) {   // the largest 2^e with bound 2^e <= limit; 1 if there is none
+  if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
+  int e;
+  frexpf(limit / bound, &e);                                              // limit / bound = m 2^e, m in [0.5, 1)
+  return ldexpf(1.f, e - 1 < -100 ? -100 : e - 1 > 100 ? 100 : e - 1);
+}
+
+// Running softmax statistics of one map over 16 more scores of a lane: m = c times the largest score, rounded, l = sum of
+// 2^(c s - m).  m is kept as it was rounded: a maximum that does not change then leaves the sum as it is, bit for bit.
+__device__ __forceinline__ float row_max(const f32x16& s) {
+  float t = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+  for (int r = 3; r < 15; r += 2) t = fmaxf(fmaxf(t, s[r]), s[r + 1]);
+  return fmaxf(t, s[15]);
+}
+
+__device__ __forceinline__ void add_stats(const f32x16& s, float c, float& m, float& l) {
+  const float t = fmaxf(row_max(s) * c, m), base = t == -INFINITY ? 0.f : t;
+  float a = 0.f, b = 0.f;           // on their own first: the long sum is rounded once for 16 terms
+#pragma unroll
+  for (int r = 0; r < 16; r += 2) {
+    a += __builtin_amdgcn_exp2f(fmaf(s[r], c, -base));
+    b += __builtin_amdgcn_exp2f(fmaf(s[r + 1], c, -base));
+  }
+  l = fmaf(l, __builtin_amdgcn_exp2f(m - base), a + b);
+  m = t;
+}
+
+__device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float l2) {
+  const float t = fmaxf(m, m2), base = t == -INFINITY ? 0.f : t;
+  l = l * __builtin_amdgcn_exp2f(m - base) + l2 * __builtin_amdgcn_exp2f(m2 - base);
+  m = t;
+}
+
+// Two sweeps over the keys.  The first finds the maximum and the sum of both maps; the second forms A = P1 - lambda P2 in 32 bits, rounds
+// it once, and needs one product with v.  With dv = 2 d this is as many products as one sweep with an accumulator per map
+// (2 d + 2 d + dv against 2 d + 2 dv per pair of tokens) and half the accumulators, and A, not P1 and P2, is rounded: where the maps
+// cancel, rounding them apart would leave an error of the size of what was cancelled.
+// A workgroup has 4 waves: 4 / KW groups of 32 queries, and KW waves that share a tile's keys.
+template <class T, int DP, int DVP>
+struct FwdShape {
+  static constexpr int P = Type<T>::planes;
+  typedef Tile<2 * DP, P> KTile;
+  typedef Tile<DVP, P> VTile;
+  static constexpr int MERGE = 2 * DVP * 128;                 // two waves' 32 x DVP sums
+  static constexpr int TILES = KTile::BYTES + VTile::BYTES;
+  static constexpr int WORDS = TILES > MERGE ? TILES : MERGE; // offset of the mask words
+  static constexpr int LDS = WORDS + WINDOW * 8;
+  static constexpr int MIN_BLOCKS = P == 3 && DP > 32 ? 1 : 2;
+};
+
+template <class T, int DP, int DVP, int KW>
+__global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void fwd_kernel(Args a) {
+  typedef FwdShape<T, DP, DVP> S;
+  typedef typename S::KTile KTile;
+  typedef typename S::VTile VTile;
+  constexpr int P = S::P, QW = 4 / KW, BQ = 32 * QW, NV = DVP / 32;
+  extern __shared__ __align__(256) char lds[];
+  char* kt = lds;
+  char* vt = lds + KTile::BYTES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
+  const int qw = wave / KW, kw = wave - qw * KW;
+  const int q_tiles = (a.N + BQ - 1) / BQ;
+  const unsigned id = die_major(blockIdx.x, gridDim.x);
+  const int bh = id / q_tiles, qt = a.causal ? q_tiles - 1 - (int)(id - bh * q_tiles) : (int)(id - bh * q_tiles);   // causal: long ones first
+  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+  const int q = qt * BQ + 32 * qw + l31;
+  const bool q_on = q < a.N;
+  const long long off = (long long)a.M - a.N;                  // causal: query q sees the keys <= q + off
+  const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
+  const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
+
+  Frag<P> qf[2][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)q * a.qn + (2ll * h + i) * a.qh, q_on, a.d, g);
+
+  KeyBits keys;
+  keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
+  keys.words = reinterpret_cast<u64*>(lds + S::WORDS);
+  keys.M = a.M;
+  keys.end = (a.M + TILE - 1) / TILE;
+  if (a.causal) {
+    const long long q_last = (qt + 1) * BQ < a.N ? (qt + 1) * BQ - 1 : a.N - 1, last = q_last + off;
+    const int e = last < 0 ? 0 : (int)(last / TILE) + 1;
+    if (e < keys.end) keys.end = e;
+  }
+  const long long wave_last = (long long)qt * BQ + 32 * qw + 31 + off;   // causal: last key that any query of the wave may see
+
+  Stage<T, 2 * DP, 2> ks;
+  Stage<T, DVP, 1> vs;
+  auto score = [&](int i, int hh) {
+    Dot<T> s;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+    return s.sum();
+  };
+  auto seen = [&](int t, u64 bits) { return a.causal ? bits & upto(q + off - (long long)t * TILE) : bits; };
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  u64 bits, bits_next;
+  keys.start(0, wave, lane);
+  int t = keys.next(0, bits, wave, lane);
+  if (t < keys.end) ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
+  while (t < keys.end) {
+    __syncthreads();
+    ks.put(kt, tid);
+    __syncthreads();
+    const int tn = keys.next(t + 1, bits_next, wave, lane);
+    if (tn < keys.end) ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
+    if (!a.causal || (long long)t * TILE <= wave_last) {
+      const u64 see = seen(t, bits);
+      const bool part = __any(see != ~0ull);
+#pragma unroll
+      for (int half = 0; half < 2 / KW; ++half) {
+        const int hh = KW == 1 ? half : kw;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x16 s = score(i, hh);
+          if (part) hide(s, see, hh, g);
+          add_stats(s, a.c, m[i], l[i]);
+        }
+      }
+    }
+    t = tn;
+    bits = bits_next;
+  }
+  float mc[2], il[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) merge_stats(m[i], l[i], __shfl_xor(m[i], 32), __shfl_xor(l[i], 32));
+  if constexpr (KW == 2) {
+    float* box = reinterpret_cast<float*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (g == 0) { box[(wave * 4 + 2 * i) * 32 + l31] = m[i]; box[(wave * 4 + 2 * i + 1) * 32 + l31] = l[i]; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int w0 = wave & ~1;
+      float m0 = box[(w0 * 4 + 2 * i) * 32 + l31], l0 = box[(w0 * 4 + 2 * i + 1) * 32 + l31];
+      merge_stats(m0, l0, box[((w0 + 1) * 4 + 2 * i) * 32 + l31], box[((w0 + 1) * 4 + 2 * i + 1) * 32 + l31]);
+      m[i] = m0;
+      l[i] = l0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // a query that sees nothing: every 2^(c s - mc) is 0
+    mc[i] = l[i] == 0.f ? INFINITY : m[i];
+    il[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+    if (a.stats != nullptr && q_on && kw == 0 && g == 0)
+      a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + q] = make_float2(mc[i], il[i]);
+  }
+  const float lam = a.lambda[h];
+  float up = 1.f;
+  if constexpr (sizeof(T) == 2 && Type<T>::planes == 1) {
+    if (__is_same(T, _Float16)) up = pow2_below(16384.f, fmaxf(1.f, fabsf(lam)));
+  }
+  const float w1 = up * il[0], w2 = up * lam * il[1];
+
+  f32x16 o[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) o[i] = zero16();
+  __syncthreads();
+  keys.start(0, wave, lane);
+  t = keys.next(0, bits, wave, lane);
+  if (t < keys.end) {
+    ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
+    vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+  }
+  while (t < keys.end) {
+    __syncthreads();
+    ks.put(kt, tid);
+    vs.put(vt, tid);
+    __syncthreads();
+    const int tn = keys.next(t + 1, bits_next, wave, lane);
+    if (tn < keys.end) {
+      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
+      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+    }
+    if (!a.causal || (long long)t * TILE <= wave_last) {
+      const u64 see = seen(t, bits);
+      const bool part = __any(see != ~0ull);
+#pragma unroll
+      for (int half = 0; half < 2 / KW; ++half) {
+        const int hh = KW == 1 ? half : kw;
+        f32x16 s1 = score(0, hh), s2 = score(1, hh);
+        if (part) { hide(s1, see, hh, g); hide(s2, see, hh, g); }
+        float p[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          p[r] = fmaf(__builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -mc[0])), w1, -w2 * __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -mc[1])));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const Frag<P> pf = pack8<T>(p + 8 * u);
+#pragma unroll
+          for (int i = 0; i < NV; ++i) accumulate<T>(o[i], VTile::cols(vt, 32 * hh + 16 * u, 32 * i, lane, DVP), pf);
+        }
+      }
+    }
+    t = tn;
+    bits = bits_next;
+  }
+  if constexpr (KW == 2) {         // the two waves' sums, one after the other
+    float* box = reinterpret_cast<float*>(lds) + (size_t)qw * NV * 16 * 64;
+    __syncthreads();
+    if (kw == 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[(i * 16 + r) * 64 + lane] = o[i][r];
+    }
+    __syncthreads();
+    if (kw == 1) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] += box[(i * 16 + r) * 64 + lane];
+  }
+  if (!q_on) return;
+  const float down = 1.f / up;
+  T* op = static_cast<T*>(a.out) + (((long long)b * a.N + q) * a.H + h) * a.dv_w;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int col = 32 * i + 2 * r + 4 * g;
+      if (col < a.dv_w) store4<T>(op + col, o[i][r] * down, o[i][r + 1] * down, o[i][r + 2] * down, o[i][r + 3] * down);
+    }
+}
+
+// A few rows against many keys: one pass over k and v, the keys split over workgroups.  The rows of a key head's group (queries x
+// heads that share it) are the columns of a 32-wide block.  The two key halves of a tile go to two waves each, which share the columns of v; every
+// such half keeps its own maximum, sum and (P v) of both maps, and `split_join` merges them.  P is at most 1 here and not yet A, so it is
+// taken in two terms (h + l): the pass waits for memory, the products are free.
+template <class T, int DP, int DVP>
+__global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void split_kernel(Args a) {
+  typedef FwdShape<T, DP, DVP> S;
+  typedef typename S::KTile KTile;
+  typedef typename S::VTile VTile;
+  constexpr int P = S::P, NV = DVP / 32, NW = (NV + 1) / 2;     // column tiles of v, per wave
+  extern __shared__ __align__(256) char lds[];
+  char* kt = lds;
+  char* vt = lds + KTile::BYTES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
+  const int hh = wave & 1, vw = wave >> 1;
+  const int group = a.H / a.Hkv, rows = a.N * group, blocks = (rows + 31) / 32;
+  unsigned id = blockIdx.x;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int rb = id % blocks, bk = id / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int row = rb * 32 + l31, n = row / group, h = hk * group + (row - n * group);
+  const bool on = row < rows;
+  const long long off = (long long)a.M - a.N;
+  const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
+  const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
+  Frag<P> qf[2][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)n * a.qn + (2ll * h + i) * a.qh, on, a.d, g);
+
+  KeyBits keys;
+  keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
+  keys.words = reinterpret_cast<u64*>(lds + S::WORDS);
+  keys.M = a.M;
+  const int tiles = (a.M + TILE - 1) / TILE, first = split * a.split_tiles;
+  keys.end = first + a.split_tiles < tiles ? first + a.split_tiles : tiles;
+
+  Stage<T, 2 * DP, 2> ks;
+  Stage<T, DVP, 1> vs;
+  f32x16 o[2][NW];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NW; ++j) o[i][j] = zero16();
+  u64 bits, bits_next;
+  keys.start(first, wave, lane);
+  int t = keys.next(first, bits, wave, lane);
+  if (t < keys.end) {
+    ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
+    vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+  }
+  while (t < keys.end) {
+    __syncthreads();
+    ks.put(kt, tid);
+    vs.put(vt, tid);
+    __syncthreads();
+    const int tn = keys.next(t + 1, bits_next, wave, lane);
+    if (tn < keys.end) {
+      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
+      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+    }
+    const u64 see = a.causal ? bits & upto(n + off - (long long)t * TILE) : bits;
+    const bool part = __any(see != ~0ull);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      Dot<T> dot;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) dot.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+      f32x16 s = dot.sum();
+      if (part) hide(s, see, hh, g);
+      float top = row_max(s) * a.c;
+      top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[i]);       // one maximum for both halves of the wave: they share a column of o
+      const float tc = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[i] - tc);
+      m[i] = top;
+      float p[16], sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -tc));
+        sum += p[r];
+      }
+      l[i] = l[i] * keep + sum;
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][j][r] *= keep;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Frag<P> pf = pack8<T>(p + 8 * u);
+        Frag<P> rest = pf;
+        if constexpr (P == 1) {
+          float q[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) q[j] = p[8 * u + j] - (float)(T)p[8 * u + j];
+          rest = pack8<T>(q);
+        }
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+          const int col = 32 * (vw + 2 * j);
+          if (col < DVP) {
+            const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, col, lane, DVP);
+            if constexpr (P == 1) accumulate<T>(o[i][j], vf, rest);
+            accumulate<T>(o[i][j], vf, pf);
+          }
+        }
+      }
+    }
+    t = tn;
+    bits = bits_next;
+  }
+  // part: [bk][row][2 splits + half][2 dv + 4]: o1, o2, m1, l1, m2, l2
+#pragma unroll
+  for (int i = 0; i < 2; ++i) l[i] += __shfl_xor(l[i], 32);
+  if (!on) return;
+  const int slots = 2 * a.splits, ld = 2 * a.dv_w + 4;
+  float* out = a.part + (((long long)bk * rows + row) * slots + 2 * split + hh) * ld;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int col = 32 * (vw + 2 * j) + 2 * r + 4 * g;
+        if (col < a.dv_w) *reinterpret_cast<f32x4*>(out + i * a.dv_w + col) = f32x4{o[i][j][r], o[i][j][r + 1], o[i][j][r + 2], o[i][j][r + 3]};
+      }
+    if (vw == 0 && g == 0) { out[2 * a.dv_w + 2 * i] = m[i]; out[2 * a.dv_w + 2 * i + 1] = l[i]; }
+  }
+}
+
+// one workgroup of 64 per (sequence, query, head): the parts of a row, in order
+template <class T>
+__global__ __launch_bounds__(64) void split_join(Args a) {
+  const int id = blockIdx.x, h = id % a.H, bn = id / a.H, n = bn % a.N, b = bn / a.N, lane = threadIdx.x;
+  const int group = a.H / a.Hkv, hk = h / group, rows = a.N * group, row = n * group + (h - hk * group);
+  const int slots = 2 * a.splits, ld = 2 * a.dv_w + 4;
+  const float* in = a.part + ((long long)(b * a.Hkv + hk) * rows + row) * slots * ld;
+  float w[2], mc[2], il[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < slots; s += 64) merge_stats(m, l, in[s * ld + 2 * a.dv_w + 2 * i], in[s * ld + 2 * a.dv_w + 2 * i + 1]);
+    for (int x = 1; x < 64; x <<= 1) merge_stats(m, l, __shfl_xor(m, x), __shfl_xor(l, x));
+    mc[i] = l == 0.f ? INFINITY : m;
+    il[i] = l == 0.f ? 0.f : 1.f / l;
+    w[i] = i == 0 ? il[0] : -a.lambda[h] * il[1];
+    if (a.stats != nullptr && lane == 0) a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + n] = make_float2(mc[i], il[i]);
+  }
+  T* out = static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w;
+  for (int c = 4 * lane; c < a.dv_w; c += 256) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < slots; ++s) {
+      const float* p = in + (long long)s * ld;
+      const float e1 = w[0] * __builtin_amdgcn_exp2f(p[2 * a.dv_w] - mc[0]), e2 = w[1] * __builtin_amdgcn_exp2f(p[2 * a.dv_w + 2] - mc[1]);
+      const f32x4 o1 = *reinterpret_cast<const f32x4*>(p + c), o2 = *reinterpret_cast<const f32x4*>(p + a.dv_w + c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += e1 * o1[r] + e2 * o2[r];
+    }
+    store4<T>(out + c, v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <class T, int DP, int DVP, int KW>
+int launch_fwd(const Args& a, hipStream_t st) {
+  typedef FwdShape<T, DP, DVP> S;
+  static LdsAttrOnce once;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
+  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
+  if (blocks > 0x7fffffffLL) return -3;
+  hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  return 0;
+}
+
+template <class T, int DP, int DVP>
+int launch_split(const Args& a, hipStream_t st) {
+  typedef FwdShape<T, DP, DVP> S;
+  static LdsAttrOnce once;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&split_kernel<T, DP, DVP>), S::LDS)) return -2;
+  const long long rows = (long long)a.N * (a.H / a.Hkv), blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32) * a.splits;
+  if (blocks > 0x7fffffffLL || (long long)a.B * a.N * a.H > 0x7fffffffLL) return -3;
+  hipLaunchKernelGGL((split_kernel<T, DP, DVP>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(64), 0, st, a);
+  return 0;
+}
+
+template <class T>
+int run_forward(const Args& a, hipStream_t st) {
+  // few workgroups: half as many queries in each, the keys of a tile shared by two waves
+  const bool few = (long long)a.B * a.H * ((a.N + 127) / 128) < 512;
+#define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return few ? launch_fwd<T, DP, DVP, 2>(a, st) : launch_fwd<T, DP, DVP, 1>(a, st);
+  SCGG_DIFF_WIDTHS(SCGG_X)
+#undef SCGG_X
+  return -1;
+}
+
+template <class T>
+int run_split(const Args& a, hipStream_t st) {
+#define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return launch_split<T, DP, DVP>(a, st);
+  SCGG_DIFF_WIDTHS(SCGG_X)
+#undef SCGG_X
+  return -1;
+}
+
+}  // namespace diffattn
+}  // namespace scgg

@@ -81,3 +81,57 @@ def test_rope_c_entry_refuses_missing_pointers():
     assert L.scgg_rope_backward(C.byref(a), None, 0, None) != 0 and "workspace" in L.scgg_last_error().decode()
     a.eps = -1.0
     assert L.scgg_rope_forward(C.byref(a), None) != 0 and "eps" in L.scgg_last_error().decode()
+
+
+def test_diff_attention_refuses():
+    f = A.diff_attention
+    q, k, v, lam = Z(2, 5, 4, 32), Z(2, 7, 4, 32), Z(2, 7, 2, 64), Z(2)
+    for bad, why in (((q[0], k, v, lam), r"B, tokens"), ((q.double(), k, v, lam), "float64"), ((q, k.half(), v, lam), "float16"),
+                     ((q, k[:1], v, lam), "go together"), ((q, k, v[:, :6], lam), "go together"), ((q, Z(2, 7, 4, 16), v, lam), "go together"),
+                     ((q[:, :, :3], k, v, lam), "3 heads"), ((q, k, v[:, :, :1], lam), "heads"), ((Z(2, 5, 6, 32), k, v, lam), "multiple"),
+                     ((q[:, :, :0], k, v, lam), "0 heads"), ((Z(2, 5, 4, 72), Z(2, 7, 4, 72), v, lam), "d = 72"), ((q[..., :4], k[..., :4], v, lam), "d = 4"),
+                     ((q, k, Z(2, 7, 2, 136), lam), "dv = 136"), ((q, k, v[..., :12], lam), "dv = 12"), ((q, k, v, lam.double()), "lam"),
+                     ((q, k, v, Z(3)), "lam"), ((q, k, v, Z(1, 2)), "lam"), ((q, k, v, lam), "GPU")):
+        refused(f, *bad, match=why)
+    refused(f, q, k, v, lam, key_mask=Z(2, 7), match="bool")
+    refused(f, q, k, v, lam, key_mask=Z(2, 6, dtype=torch.bool), match="is needed")
+    refused(f, q, k, v, lam, key_mask=[True], match="bool")
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        refused(f, q, k, v, lam, scale=scale, match="scale")
+
+
+def diff_args(**kw):
+    a = _lib.DiffAttentionArgs()
+    a.B, a.N, a.M, a.H, a.Hkv, a.d, a.dv, a.scale = 2, 3, 4, 2, 1, 32, 64, 0.1
+    for n in ("q", "k", "v", "lambda", "out", "stats", "dout", "dq", "dk", "dv_out", "dlambda"):
+        setattr(a, n, 4096)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,why", [(dict(dtype=-1), "dtype"), (dict(N=-1), "shape"), (dict(H=3, Hkv=2), "heads"), (dict(Hkv=0), "heads"), (dict(d=72), "d = 72"),
+                                    (dict(d=12), "d = 12"), (dict(dv=0), "dv = 0"), (dict(dv=136), "dv = 136"), (dict(scale=0.0), "scale"),
+                                    (dict(scale=float("nan")), "scale"), (dict(M=2 ** 31 - 1), "too many"), (dict(B=2 ** 20, H=2 ** 12), "too many")])
+def test_diff_c_entry_refuses(kw, why):
+    L, a = _lib.lib(), diff_args(**kw)
+    assert L.scgg_diff_attention_forward(C.byref(a), None, 0, None) != 0 and why in L.scgg_last_error().decode()
+    assert L.scgg_diff_attention_backward(C.byref(a), None, 0, None) != 0
+    assert L.scgg_diff_attention_forward_workspace_bytes(C.byref(a)) == 0 and L.scgg_diff_attention_backward_workspace_bytes(C.byref(a)) == 0
+
+
+def test_diff_c_entry_refuses_pointers_alignment_and_workspace():
+    L = _lib.lib()
+    assert L.scgg_diff_attention_forward(None, None, 0, None) != 0
+    for n in ("q", "k", "v", "lambda", "out"):
+        assert L.scgg_diff_attention_forward(C.byref(diff_args(**{n: None})), None, 0, None) != 0 and "null" in L.scgg_last_error().decode()
+    for n in ("dout", "dq", "dk", "dv_out", "dlambda", "stats"):
+        assert L.scgg_diff_attention_backward(C.byref(diff_args(**{n: None})), 4096, 1 << 30, None) != 0 and "null" in L.scgg_last_error().decode()
+    for kw in (dict(q=4104), dict(k_stride_n=2), dict(v_stride_b=1)):
+        assert L.scgg_diff_attention_forward(C.byref(diff_args(**kw)), None, 0, None) != 0 and "16 bytes" in L.scgg_last_error().decode()
+    assert L.scgg_diff_attention_backward(C.byref(diff_args(dout_stride_h=2)), 4096, 1 << 30, None) != 0 and "dout" in L.scgg_last_error().decode()
+    a = diff_args(N=1, M=100000)
+    need = L.scgg_diff_attention_forward_workspace_bytes(C.byref(a))
+    assert need > 0
+    assert L.scgg_diff_attention_forward(C.byref(a), 4096, need - 1, None) != 0 and "workspace" in L.scgg_last_error().decode()
+    assert L.scgg_diff_attention_backward(C.byref(a), None, 0, None) != 0 and "workspace" in L.scgg_last_error().decode()
