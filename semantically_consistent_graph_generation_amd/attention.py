@@ -60,10 +60,10 @@ def _dense_rows(t):
 
 
 def _aligned_rows(t):
-    """Dense rows that start at multiples of 16 bytes; a copy where they do not."""
+    """Dense rows that start at multiples of 16 bytes, 64 of them (and two heads) within 2 GiB; a copy where they do not."""
     t = _dense_rows(t)
-    size = t.element_size()
-    if t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in _strides(t)):
+    size, (b, n, h) = t.element_size(), _strides(t)
+    if (t.data_ptr() | b * size | n * size | h * size) % 16 == 0 and (63 * n + h + t.shape[3]) * size < 2 ** 31 - 32:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -128,10 +128,8 @@ template <class T>
 __device__ __forceinline__ void pack2(float x, float y, unsigned (&out)[Type<T>::planes]) {
   if constexpr (Type<T>::planes == 1) {
     typedef T t2 __attribute__((ext_vector_type(2)));
-    t2 v;
-    v[0] = (T)x;
-    v[1] = (T)y;
-    out[0] = __builtin_bit_cast(unsigned, v);
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    out[0] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2{x, y}), t2));   // one conversion for both, to nearest
   } else {                         // x = h + m + l by truncation: exact
     unsigned u = __float_as_uint(x), w = __float_as_uint(y);
     out[0] = __builtin_amdgcn_perm(w, u, 0x07060302u);
@@ -159,11 +157,21 @@ __device__ __forceinline__ Frag<Type<T>::planes> pack8(const float* x) {
   return f;
 }
 
+// Loads of a tile go through a buffer descriptor: a 64-bit base in scalar registers for the tile, a 32-bit byte offset per lane, and
+// an offset past the descriptor's 2 GiB gives zeros without a branch.
+constexpr unsigned NOWHERE = 0x80000000u;
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7fffffff, 0x00027000);
+}
+__device__ __forceinline__ u32x4 buffer_load(Buffer b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0); }
+
 // 8 elements as they lie in memory
 template <class T>
 struct Raw {
   u32x4 a;
   __device__ __forceinline__ void load(const T* p) { a = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void load(Buffer b, unsigned at) { a = buffer_load(b, at); }
   __device__ __forceinline__ void clear() { a = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ Frag<1> frag() const { return Frag<1>{{a}}; }
 };
@@ -171,6 +179,10 @@ template <>
 struct Raw<float> {
   f32x4 a, b;
   __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const f32x4*>(p); b = *reinterpret_cast<const f32x4*>(p + 4); }
+  __device__ __forceinline__ void load(Buffer f, unsigned at) {
+    a = __builtin_bit_cast(f32x4, buffer_load(f, at));
+    b = __builtin_bit_cast(f32x4, buffer_load(f, at == NOWHERE ? at : at + 16));
+  }
   __device__ __forceinline__ void clear() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ Frag<3> frag() const {
     const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -283,6 +295,23 @@ __device__ __forceinline__ void hide(f32x16& s, u64 bits, int hh, int g) {
   for (int r = 0; r < 16; ++r) s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1u ? s[r] : -INFINITY;
 }
 
+// P = 2^(c s - m) il: one exponent that holds il too where P is rounded to 16 bits (m - log2(il) is off by 2^-24 of itself), the product
+// where it is not
+template <class T>
+struct Prob {
+  static constexpr bool folded = Type<T>::planes == 1;
+  float m, f;
+  __device__ __forceinline__ Prob() {}
+  __device__ __forceinline__ Prob(float mc, float il, float factor) {     // factor: a power of two
+    m = folded ? (il == 0.f ? INFINITY : mc - __builtin_amdgcn_logf(il * factor)) : mc;
+    f = folded ? 1.f : il * factor;
+  }
+  __device__ __forceinline__ float operator()(float s, float c) const {
+    const float e = __builtin_amdgcn_exp2f(fmaf(s, c, -m));
+    return folded ? e : e * f;
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ staging
 // A tile's rows into registers, 8 elements a piece, and from there into LDS: the loads of the next tile are under way while
 // this one is used.  Rows whose bit is off and columns from `width` on are zeros, whatever memory holds there.
@@ -292,13 +321,23 @@ struct Stage {
   static_assert(TILE * PIECES % NT == 0, "whole pieces per thread");
   typedef Tile<W, Type<T>::planes> tile;
   Raw<T> raw[PER];
-  __device__ __forceinline__ void load(const T* base, long long row_stride, long long head_stride, long long row0, u64 bits, int width, int tid) {
+  unsigned at[PER];                                        // byte offset of each piece from the tile's first row
+  __device__ __forceinline__ void init(long long row_stride, long long head_stride, int width, int tid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int i = tid + j * NT, row = i / PIECES, pc = i - row * PIECES;
       const int head = HEADS == 1 ? 0 : pc / (HW / 8), col = (pc - head * (HW / 8)) * 8;
-      if (((bits >> row) & 1) && col < width) raw[j].load(base + (row0 + row) * row_stride + head * head_stride + col);
-      else raw[j].clear();
+      at[j] = col < width ? (unsigned)((row * row_stride + head * head_stride + col) * (long long)sizeof(T)) : NOWHERE;
+    }
+  }
+  __device__ __forceinline__ void load(const T* first_row, u64 bits, int tid) {
+    const Buffer b = buffer(first_row);
+    if (bits == ~0ull) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) raw[j].load(b, at[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) raw[j].load(b, ((bits >> ((tid + j * NT) / PIECES)) & 1) ? at[j] : NOWHERE);
     }
   }
   __device__ __forceinline__ void put(char* lds, int tid) const {
@@ -327,12 +366,7 @@ __device__ __forceinline__ void load_rows(Frag<Type<T>::planes> (&f)[W / 16], co
 template <class T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
   typedef T t4 __attribute__((ext_vector_type(4)));
-  t4 v;
-  v[0] = (T)a;
-  v[1] = (T)b;
-  v[2] = (T)c;
-  v[3] = (T)d;
-  *reinterpret_cast<t4*>(p) = v;
+  *reinterpret_cast<t4*>(p) = __builtin_convertvector((f32x4{a, b, c, d}), t4);
 }
 
 // Work index -> place: consecutive workgroups go to the 8 dies in turn, so a die takes a contiguous stretch of the work (the tiles

@@ -42,12 +42,20 @@ bool aligned(const scgg_diff_attention_args* p, const void* base, int64_t sb, in
   return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)((sb | sn | sh) * size)) & 15) == 0;
 }
 
+// a tile's rows lie within the 2 GiB that a 32-bit offset reaches
+bool near(const scgg_diff_attention_args* p, int64_t sn, int64_t sh, int width) {
+  const int64_t size = p->dtype == SCGG_F32 ? 4 : 2;
+  return sn >= 0 && sh >= 0 && sn < (1ll << 40) && sh < (1ll << 40) && ((TILE - 1) * sn + sh + width) * size < 0x7fffffffll - 16;
+}
+
 int check_inputs(const scgg_diff_attention_args* p, const char* what) {
   const bool queries = p->B > 0 && p->N > 0, keys = p->B > 0 && p->M > 0;
   if ((queries && !p->q) || (keys && (!p->k || !p->v)) || !p->lambda) return fail("%s: null argument", what);
   if ((queries && !aligned(p, p->q, p->q_stride_b, p->q_stride_n, p->q_stride_h)) ||
       (keys && (!aligned(p, p->k, p->k_stride_b, p->k_stride_n, p->k_stride_h) || !aligned(p, p->v, p->v_stride_b, p->v_stride_n, p->v_stride_h))))
     return fail("%s: bases and strides of q, k and v have to be multiples of 16 bytes", what);
+  if ((queries && !near(p, p->q_stride_n, p->q_stride_h, p->d)) || (keys && (!near(p, p->k_stride_n, p->k_stride_h, p->d) || !near(p, p->v_stride_n, 0, p->dv))))
+    return fail("%s: rows of q, k and v have to lie less than 2 GiB / 64 apart", what);
   return 0;
 }
 
@@ -131,6 +139,7 @@ extern "C" int scgg_diff_attention_backward(const scgg_diff_attention_args* p, v
   if ((queries && (!p->dout || !p->dq || !p->stats)) || (keys && (!p->dk || !p->dv_out)) || !p->dlambda) return fail("%s: null argument", what);
   if (queries && !aligned(p, p->dout, p->dout_stride_b, p->dout_stride_n, p->dout_stride_h))
     return fail("%s: base and strides of dout have to be multiples of 16 bytes", what);
+  if (queries && !near(p, p->dout_stride_n, 0, p->dv)) return fail("%s: rows of dout have to lie less than 2 GiB / 64 apart", what);
   Args a = make(p);
   const size_t need = delta_bytes(a);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);

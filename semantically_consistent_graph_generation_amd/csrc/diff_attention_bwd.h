@@ -46,14 +46,13 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
 
   Frag<P> qf[2][DP / 16], gf[DVP / 16];
-  float mc[2], il[2];
+  Prob<T> prob[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)q * a.qn + (2ll * h + i) * a.qh, q_on, a.d, g);
     float2 st = make_float2(INFINITY, 0.f);
     if (q_on) st = a.stats[((long long)bh * 2 + i) * a.N + q];
-    mc[i] = st.x;
-    il[i] = st.y;
+    prob[i] = Prob<T>(st.x, st.y, 1.f);
   }
   load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on, a.dv_w, g);
 
@@ -71,6 +70,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
 
   Stage<T, 2 * DP, 2> ks;
   Stage<T, DVP, 1> vs;
+  ks.init(a.kn, a.kh, a.d, tid);
+  vs.init(a.vn, 0, a.dv_w, tid);
   auto score = [&](int i, int hh) {
     Dot<T> s;
 #pragma unroll
@@ -88,8 +89,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
     keys.start(0, wave, lane);
     t = keys.next(0, bits, wave, lane);
     if (t < keys.end) {
-      ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
-      vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+      ks.load(kp + (long long)t * TILE * a.kn, bits, tid);
+      vs.load(vp + (long long)t * TILE * a.vn, bits, tid);
     }
   };
   auto advance = [&](int t, u64& bits_next) {       // this tile into LDS, the next one's loads under way
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
     __syncthreads();
     const int tn = keys.next(t + 1, bits_next, wave, lane);
     if (tn < keys.end) {
-      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
-      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+      ks.load(kp + (long long)tn * TILE * a.kn, bits_next, tid);
+      vs.load(vp + (long long)tn * TILE * a.vn, bits_next, tid);
     }
     return tn;
   };
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
           if (part) hide(s, see, hh, g);
           float sum = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
-          delta[i] = fmaf(sum, il[i], delta[i]);
+          for (int r = 0; r < 16; ++r) sum = fmaf(prob[i](s[r], a.c), dp[r], sum);
+          delta[i] += sum;
         }
         if (__is_same(T, _Float16)) {
 #pragma unroll
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   }
   float up = 1.f;                                   // |dS| <= 2 max(1, |lambda|) max |dP|
   if (__is_same(T, _Float16)) up = pow2_below(16384.f, 2.f * fmaxf(1.f, fabsf(lam)) * top);
-  const float w1 = up * il[0], w2 = -up * lam * il[1];
+  const float w[2] = {up, -up * lam}, wd[2] = {-w[0] * delta[0], -w[1] * delta[1]};
 
   f32x16 o[2][ND];
 #pragma unroll
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
           if (part) hide(s, see, hh, g);
           float ds[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])) * (i == 0 ? w1 : w2) * (dp[r] - delta[i]);
+          for (int r = 0; r < 16; ++r) ds[r] = prob[i](s[r], a.c) * fmaf(dp[r], w[i], wd[i]);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const Frag<P> df = pack8<T>(ds + 8 * u);
@@ -236,12 +237,13 @@ struct DkvShape {
   static constexpr int MERGE = 2 * (2 * ND + NV) * 16 * 64 * 4;
   static constexpr int ROWS = TILES > MERGE ? TILES : MERGE;      // offset of the rows' statistics [6][TILE]
   static constexpr int LDS = ROWS + 6 * TILE * 4;
+  static constexpr int MIN_BLOCKS = P == 1 && DP <= 32 ? 2 : 1;
 };
 
 // Over keys: a wave keeps 32 of them (k1, k2 and v as operands, dK1, dK2 and dV as sums) and the queries of all heads that share the key
 // head stream by.  4 / QW groups of 32 keys, QW waves that share a tile's queries.
 template <class T, int DP, int DVP, int QW>
-__global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void dkv_kernel(Args a) {
   typedef DkvShape<T, DP, DVP> S;
   typedef typename S::QTile QTile;
   typedef typename S::GTile GTile;
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
   extern __shared__ __align__(256) char lds[];
   char* qt = lds;
   char* gt = lds + QTile::BYTES;
-  float* rowst = reinterpret_cast<float*>(lds + S::ROWS);          // mc1, il1, mc2, il2, delta1, delta2 of the tile's queries
+  float* rowst = reinterpret_cast<float*>(lds + S::ROWS);          // of the tile's queries: m and il of both maps (Prob), - w_i delta_i
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
   const int kg = wave / QW, qw = wave - kg * QW;
   const int k_tiles = (a.M + BK - 1) / BK, group = a.H / a.Hkv;
@@ -294,36 +296,49 @@ __global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
     const long long q_first = (long long)kt * BK - off;
     if (q_first > 0) t_first = q_first / TILE < n_tiles ? (int)(q_first / TILE) : n_tiles;
   }
-  const int steps = (n_tiles - t_first) * group;
   // a workgroup whose keys are all hidden has nothing to sum
   const bool any = __syncthreads_or(k_on);
   Stage<T, 2 * DP, 2> qs;
   Stage<T, DVP, 1> gs;
+  qs.init(a.qn, a.qh, a.d, tid);
+  gs.init(a.gn, 0, a.dv_w, tid);
   float2 rs;
-  auto load = [&](int step) {
-    const int hg = step / (n_tiles - t_first), t = t_first + step - hg * (n_tiles - t_first), h = hk * group + hg;
+  float rlam;
+  auto load = [&](int hg, int t) {
+    const int h = hk * group + hg;
     const long long left = (long long)a.N - (long long)t * TILE;
     const u64 bits = left >= TILE ? ~0ull : (1ull << left) - 1;
-    qs.load(static_cast<const T*>(a.q) + b * a.qb + 2ll * h * a.qh, a.qn, a.qh, (long long)t * TILE, bits, a.d, tid);
-    gs.load(static_cast<const T*>(a.dout) + b * a.gb + (long long)h * a.gh, a.gn, 0, (long long)t * TILE, bits, a.dv_w, tid);
-    const int n = t * TILE + lane;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
     const long long bh = (long long)b * a.H + h;
+    const int n = t * TILE + lane;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
+    rlam = a.lambda[h];
     rs = wave < 2 ? make_float2(INFINITY, 0.f) : make_float2(0.f, 0.f);
     if (n < a.N) {
       if (wave < 2) rs = a.stats[(bh * 2 + wave) * a.N + n];
       else if (wave == 2) rs = make_float2(a.delta[bh * 3 * a.N + n], a.delta[(bh * 3 + 1) * a.N + n]);
     }
+    qs.load(static_cast<const T*>(a.q) + b * a.qb + 2ll * h * a.qh + (long long)t * TILE * a.qn, bits, tid);
+    gs.load(static_cast<const T*>(a.dout) + b * a.gb + (long long)h * a.gh + (long long)t * TILE * a.gn, bits, tid);
   };
-  if (any && steps > 0) load(0);
-  for (int step = 0; any && step < steps; ++step) {
+  int hg = 0, t = t_first;
+  const bool work = any && t_first < n_tiles;
+  if (work) load(hg, t);
+  while (work && hg < group) {
     __syncthreads();
     qs.put(qt, tid);
     gs.put(gt, tid);
-    if (wave < 3) { rowst[2 * wave * TILE + lane] = rs.x; rowst[(2 * wave + 1) * TILE + lane] = rs.y; }
+    const float lam = rlam, w1 = up_s, w2 = -lam * up_s;
+    if (wave < 2) {
+      const Prob<T> pr(rs.x, rs.y, 1.f);
+      rowst[2 * wave * TILE + lane] = pr.m;
+      if (!Prob<T>::folded) rowst[(2 * wave + 1) * TILE + lane] = pr.f;
+    } else if (wave == 2) {
+      rowst[4 * TILE + lane] = -w1 * rs.x;
+      rowst[5 * TILE + lane] = -w2 * rs.y;
+    }
     __syncthreads();
-    const int hg = step / (n_tiles - t_first), t = t_first + step - hg * (n_tiles - t_first);
-    if (step + 1 < steps) load(step + 1);
-    const float lam = a.lambda[hk * group + hg];
+    int t_next = t + 1, hg_next = hg;
+    if (t_next == n_tiles) { t_next = t_first; ++hg_next; }
+    if (hg_next < group) load(hg_next, t_next);
 #pragma unroll
     for (int half = 0; half < 2 / QW; ++half) {
       const int hh = QW == 1 ? half : qw;
@@ -335,29 +350,40 @@ __global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
         for (int c = 0; c < DP / 16; ++c) s.add(QTile::rows(qt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), kf[i][c]);
         return s.sum();
       };
-      const f32x16 s1 = score(0), s2 = score(1);
+      f32x16 s1 = score(0), s2 = score(1);
       Dot<T> dot;
 #pragma unroll
       for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh + l31, 2 * c + g), vf[c]);
       const f32x16 dp = dot.sum();
-      const bool cut = a.causal && (long long)t * TILE + 32 * hh + off < (long long)kt * BK + 32 * kg + 31;
+      if (a.causal && (long long)t * TILE + 32 * hh + off < (long long)kt * BK + 32 * kg + 31) {   // some query of these does not see some key
+        const long long from = key - off - (long long)t * TILE - 32 * hh;                             // the first that sees the lane's
+        const int first = from < 0 ? 0 : from > 32 ? 32 : (int)from;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool on = 8 * (r >> 2) + 4 * g + (r & 3) >= first;
+          s1[r] = on ? s1[r] : -INFINITY;
+          s2[r] = on ? s2[r] : -INFINITY;
+        }
+      }
       float pa[16], d1[16], d2[16];
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int row = 32 * hh + 8 * r4 + 4 * g;
-        const f32x4 m1 = *reinterpret_cast<const f32x4*>(rowst + row), i1 = *reinterpret_cast<const f32x4*>(rowst + TILE + row),
-                    m2 = *reinterpret_cast<const f32x4*>(rowst + 2 * TILE + row), i2 = *reinterpret_cast<const f32x4*>(rowst + 3 * TILE + row),
+        const f32x4 m1 = *reinterpret_cast<const f32x4*>(rowst + row), m2 = *reinterpret_cast<const f32x4*>(rowst + 2 * TILE + row),
                     e1 = *reinterpret_cast<const f32x4*>(rowst + 4 * TILE + row), e2 = *reinterpret_cast<const f32x4*>(rowst + 5 * TILE + row);
+        f32x4 i1, i2;
+        if (!Prob<T>::folded) {
+          i1 = *reinterpret_cast<const f32x4*>(rowst + TILE + row);
+          i2 = *reinterpret_cast<const f32x4*>(rowst + 3 * TILE + row);
+        }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int r = 4 * r4 + x;
-          float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -m1[x])) * i1[x];
-          float p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -m2[x])) * i2[x];
-          if (cut && key > t * (long long)TILE + row + x + off) p1 = p2 = 0.f;
-          p2 *= -lam;
-          pa[r] = (p1 + p2) * up_a;
-          d1[r] = p1 * (dp[r] - e1[x]) * up_s;
-          d2[r] = p2 * (dp[r] - e2[x]) * up_s;
+          float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -m1[x])), p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -m2[x]));
+          if (!Prob<T>::folded) { p1 *= i1[x]; p2 *= i2[x]; }
+          pa[r] = fmaf(-lam, p2, p1) * up_a;
+          d1[r] = p1 * fmaf(dp[r], w1, e1[x]);
+          d2[r] = p2 * fmaf(dp[r], w2, e2[x]);
         }
       }
 #pragma unroll
@@ -373,6 +399,8 @@ __global__ __launch_bounds__(THREADS, 1) void dkv_kernel(Args a) {
         }
       }
     }
+    t = t_next;
+    hg = hg_next;
   }
   if constexpr (QW == 2) {
     float* box = reinterpret_cast<float*>(lds) + (size_t)kg * (2 * ND + NV) * 16 * 64;

@@ -97,6 +97,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
 
   Stage<T, 2 * DP, 2> ks;
   Stage<T, DVP, 1> vs;
+  ks.init(a.kn, a.kh, a.d, tid);
+  vs.init(a.vn, 0, a.dv_w, tid);
   auto score = [&](int i, int hh) {
     Dot<T> s;
 #pragma unroll
@@ -109,13 +111,13 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
   u64 bits, bits_next;
   keys.start(0, wave, lane);
   int t = keys.next(0, bits, wave, lane);
-  if (t < keys.end) ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
+  if (t < keys.end) ks.load(kp + (long long)t * TILE * a.kn, bits, tid);
   while (t < keys.end) {
     __syncthreads();
     ks.put(kt, tid);
     __syncthreads();
     const int tn = keys.next(t + 1, bits_next, wave, lane);
-    if (tn < keys.end) ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
+    if (tn < keys.end) ks.load(kp + (long long)tn * TILE * a.kn, bits_next, tid);
     if (!a.causal || (long long)t * TILE <= wave_last) {
       const u64 see = seen(t, bits);
       const bool part = __any(see != ~0ull);
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
   if constexpr (sizeof(T) == 2 && Type<T>::planes == 1) {
     if (__is_same(T, _Float16)) up = pow2_below(16384.f, fmaxf(1.f, fabsf(lam)));
   }
-  const float w1 = up * il[0], w2 = up * lam * il[1];
+  const Prob<T> p1(mc[0], il[0], up), p2(mc[1], il[1], up);
 
   f32x16 o[NV];
 #pragma unroll
@@ -173,8 +175,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
   keys.start(0, wave, lane);
   t = keys.next(0, bits, wave, lane);
   if (t < keys.end) {
-    ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
-    vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+    ks.load(kp + (long long)t * TILE * a.kn, bits, tid);
+    vs.load(vp + (long long)t * TILE * a.vn, bits, tid);
   }
   while (t < keys.end) {
     __syncthreads();
@@ -183,8 +185,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
     __syncthreads();
     const int tn = keys.next(t + 1, bits_next, wave, lane);
     if (tn < keys.end) {
-      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
-      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+      ks.load(kp + (long long)tn * TILE * a.kn, bits_next, tid);
+      vs.load(vp + (long long)tn * TILE * a.vn, bits_next, tid);
     }
     if (!a.causal || (long long)t * TILE <= wave_last) {
       const u64 see = seen(t, bits);
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
         float p[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          p[r] = fmaf(__builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -mc[0])), w1, -w2 * __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -mc[1])));
+          p[r] = fmaf(-lam, p2(s2[r], a.c), p1(s1[r], a.c));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const Frag<P> pf = pack8<T>(p + 8 * u);
@@ -276,6 +278,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
 
   Stage<T, 2 * DP, 2> ks;
   Stage<T, DVP, 1> vs;
+  ks.init(a.kn, a.kh, a.d, tid);
+  vs.init(a.vn, 0, a.dv_w, tid);
   f32x16 o[2][NW];
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -286,8 +290,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   keys.start(first, wave, lane);
   int t = keys.next(first, bits, wave, lane);
   if (t < keys.end) {
-    ks.load(kp, a.kn, a.kh, (long long)t * TILE, bits, a.d, tid);
-    vs.load(vp, a.vn, 0, (long long)t * TILE, bits, a.dv_w, tid);
+    ks.load(kp + (long long)t * TILE * a.kn, bits, tid);
+    vs.load(vp + (long long)t * TILE * a.vn, bits, tid);
   }
   while (t < keys.end) {
     __syncthreads();
@@ -296,8 +300,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
     __syncthreads();
     const int tn = keys.next(t + 1, bits_next, wave, lane);
     if (tn < keys.end) {
-      ks.load(kp, a.kn, a.kh, (long long)tn * TILE, bits_next, a.d, tid);
-      vs.load(vp, a.vn, 0, (long long)tn * TILE, bits_next, a.dv_w, tid);
+      ks.load(kp + (long long)tn * TILE * a.kn, bits_next, tid);
+      vs.load(vp + (long long)tn * TILE * a.vn, bits_next, tid);
     }
     const u64 see = a.causal ? bits & upto(n + off - (long long)t * TILE) : bits;
     const bool part = __any(see != ~0ull);
