@@ -11,9 +11,7 @@
 // leading partial products, which keeps fp32's accuracy at 2.7 times the rate of the fp32 matrix instructions.  A tile in LDS has a plane per
 // term, so the kernels are the same for all types.
 //
-// Tiles in LDS: 64 rows (keys, or queries in the dK / dV kernel) of 64 m bytes, with the 16-byte chunks of a row permuted by
-// the row: the row-wise reads (b128: 16 rows at one chunk) and the transposing ones (tr_b64: 4 rows at 32 columns) then both meet
-// every bank once.
+// Tiles in LDS: 64 rows (keys, or queries in the dK / dV kernel), read row-wise (b128) and transposed (tr_b64).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -44,11 +42,11 @@ struct Args {
   void *out, *dq, *dk, *dv;
   float2* stats;                  // [B,H,2,N]: scale log2(e) max, 1 / sum
   float* delta;                   // [B,H,2,N]: sum_j P_i dP
-  float* part;                    // split forward: partial results (split_kernel)
+  float* part;                    // partial results of the splits (split_kernel, dkv_kernel)
   long long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh, mb;
   float scale, c;                 // c = scale log2(e)
   int B, N, M, H, Hkv, d, dv_w, causal;
-  int splits, split_tiles;        // split forward: workgroups along the keys and the tiles each of them takes
+  int splits, split_tiles;        // forward: workgroups along the keys and the tiles each of them takes; dkv_kernel: along the queries
 };
 
 // ------------------------------------------------------------------------------------------------ element types
@@ -191,45 +189,48 @@ struct Raw<float> {
 };
 
 // ------------------------------------------------------------------------------------------------ tiles in LDS
-// A tile of `ROWS` rows and W columns, P planes; row = 2 W bytes (a multiple of 64)
+// A tile of `ROWS` rows and W columns, P planes.  A row is an odd number of 64-byte groups, so four rows in a row start 16 banks
+// apart, and the four chunks of a group are permuted by row / 4: 16 rows at one chunk meet every bank once, and so do 4 rows at
+// 32 columns.  The permutation stays within a group: all reads of a lane are two addresses and constant offsets.
 template <int W, int P, int ROWS = TILE>
 struct Tile {
-  static constexpr int ROW = 2 * W, PLANE = ROWS * ROW, BYTES = P * PLANE;
-  static_assert(ROW % 64 == 0, "rows of whole 64-byte groups");
+  static constexpr int GROUPS = W / 32, ROW = 64 * (GROUPS % 2 == 0 ? GROUPS + 1 : GROUPS), PLANE = ROWS * ROW, BYTES = P * PLANE;
+  static_assert(W % 32 == 0, "rows of whole 64-byte groups");
   static __device__ __forceinline__ int place(int row, int chunk) {    // byte offset of a row's 16-byte chunk
-    int c;
-    if constexpr (ROW % 256 == 0) c = chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
-    else if constexpr (ROW % 128 == 0) c = chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
-    else c = chunk ^ ((row >> 2) & 3);
-    return row * ROW + c * 16;
+    return row * ROW + 16 * (chunk ^ ((row >> 2) & 3));
   }
   static __device__ __forceinline__ void put(char* base, int row, int chunk, const Frag<P>& f) {
 #pragma unroll
     for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(base + p * PLANE + place(row, chunk)) = f.p[p];
   }
-  // operand whose row / column index is the tile's row and whose slots are columns 8 chunk .. 8 chunk + 7
-  static __device__ __forceinline__ Frag<P> rows(const char* base, int row, int chunk) {
+  // operand whose row / column index is the tile's row `row0 + (lane & 31)` and whose slots are columns 16 c + 8 g ..
+  static __device__ __forceinline__ Frag<P> rows(const char* base, int row0, int c, int lane) {
+    const int row = lane & 31, g = lane >> 5, at = row * ROW + 16 * (g ^ ((row >> 2) & 3));
     Frag<P> f;
 #pragma unroll
-    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const u32x4*>(base + p * PLANE + place(row, chunk));
+    for (int p = 0; p < P; ++p)
+      f.p[p] = *reinterpret_cast<const u32x4*>(base + (at ^ ((c & 1) * 32)) + p * PLANE + row0 * ROW + (c >> 1) * 64);
     return f;
   }
   // operand whose row / column index is the tile's column col0 + (lane & 31) and whose slots are the 16 rows from row0 in
   // the order of a result's rows.  `last`: first column behind the ones that matter; lanes behind it read a neighbour's
   static __device__ __forceinline__ Frag<P> cols(const char* base, int row0, int col0, int lane, int last) {
     const int i = lane & 15, sub = (lane >> 4) & 1, g = lane >> 5;
-    int col = col0 + 16 * sub;
-    if (col >= last) col = col0;
-    col += 4 * (i & 3);
     Frag<P> f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = row0 + 8 * u + 4 * g + (i >> 2);
-        const char* at = base + p * PLANE + place(row, col >> 3) + 2 * (col & 7);
+        int at;
+        if (col0 % 32 == 0 && col0 + 32 <= last) {
+          const int lane_at = (4 * g + (i >> 2)) * ROW + 16 * ((2 * sub + ((i & 3) >> 1)) ^ g) + 8 * (i & 1);
+          at = (lane_at ^ (u * 32)) + (row0 + 8 * u) * ROW + (col0 >> 5) * 64;
+        } else {
+          const int col = (col0 + 16 * sub >= last ? col0 : col0 + 16 * sub) + 4 * (i & 3), row = 8 * u + 4 * g + (i >> 2);
+          at = row0 * ROW + place(row, col >> 3) + 2 * (col & 7);
+        }
         const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)at));
+            (__attribute__((address_space(3))) s16x4*)(base + p * PLANE + at)));
         f.p[p][2 * u] = w[0];
         f.p[p][2 * u + 1] = w[1];
       }
@@ -315,19 +316,18 @@ struct Prob {
 // ------------------------------------------------------------------------------------------------ staging
 // A tile's rows into registers, 8 elements a piece, and from there into LDS: the loads of the next tile are under way while
 // this one is used.  Rows whose bit is off and columns from `width` on are zeros, whatever memory holds there.
-template <class T, int W, int HEADS, int NT = THREADS>   // HEADS heads of W / HEADS columns side by side in a row
+template <class T, int W, int HEADS, int ROWS = TILE>     // HEADS heads of W / HEADS columns side by side in a row
 struct Stage {
-  static constexpr int PIECES = W / 8, PER = TILE * PIECES / NT, HW = W / HEADS;
-  static_assert(TILE * PIECES % NT == 0, "whole pieces per thread");
-  typedef Tile<W, Type<T>::planes> tile;
+  static constexpr int PIECES = W / 8, ALL = ROWS * PIECES, PER = (ALL + THREADS - 1) / THREADS, HW = W / HEADS;
+  typedef Tile<W, Type<T>::planes, ROWS> tile;
   Raw<T> raw[PER];
   unsigned at[PER];                                        // byte offset of each piece from the tile's first row
   __device__ __forceinline__ void init(long long row_stride, long long head_stride, int width, int tid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int i = tid + j * NT, row = i / PIECES, pc = i - row * PIECES;
+      const int i = tid + j * THREADS, row = i / PIECES, pc = i - row * PIECES;
       const int head = HEADS == 1 ? 0 : pc / (HW / 8), col = (pc - head * (HW / 8)) * 8;
-      at[j] = col < width ? (unsigned)((row * row_stride + head * head_stride + col) * (long long)sizeof(T)) : NOWHERE;
+      at[j] = i < ALL && col < width ? (unsigned)((row * row_stride + head * head_stride + col) * (long long)sizeof(T)) : NOWHERE;
     }
   }
   __device__ __forceinline__ void load(const T* first_row, u64 bits, int tid) {
@@ -337,14 +337,14 @@ struct Stage {
       for (int j = 0; j < PER; ++j) raw[j].load(b, at[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) raw[j].load(b, ((bits >> ((tid + j * NT) / PIECES)) & 1) ? at[j] : NOWHERE);
+      for (int j = 0; j < PER; ++j) raw[j].load(b, ((bits >> ((tid + j * THREADS) / PIECES)) & 1) ? at[j] : NOWHERE);
     }
   }
   __device__ __forceinline__ void put(char* lds, int tid) const {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int i = tid + j * NT, row = i / PIECES, pc = i - row * PIECES;
-      tile::put(lds, row, pc, raw[j].frag());
+      const int i = tid + j * THREADS, row = i / PIECES, pc = i - row * PIECES;
+      if (ALL % THREADS == 0 || i < ALL) tile::put(lds, row, pc, raw[j].frag());
     }
   }
 };

@@ -87,7 +87,19 @@ void plan_split(Args& a) {
 size_t part_bytes(const Args& a) {
   return a.splits == 0 ? 0 : (size_t)a.B * a.H * a.N * 2 * a.splits * (2 * a.dv_w + 4) * sizeof(float);
 }
-size_t delta_bytes(const Args& a) { return (size_t)a.B * a.H * 3 * a.N * sizeof(float); }
+// Queries split over workgroups in the dK / dV kernel: where the keys alone give fewer than two workgroups to each CU, and there are tiles to
+// split.  Each split writes its sums in 32 bits and they are read again, so there are four at most.
+void plan_dkv(Args& a) {
+  const long long blocks = (long long)a.B * a.Hkv * ((a.M + 127) / 128), tiles = (long long)((a.N + TILE - 1) / TILE) * (a.H / a.Hkv);
+  long long s = blocks > 0 ? 512 / blocks : 1;
+  if (s > 4) s = 4;
+  if (s > tiles / 4) s = tiles / 4;
+  a.splits = s < 1 ? 1 : (int)s;
+}
+size_t dkv_part_bytes(const Args& a) {
+  return a.splits <= 1 ? 0 : (size_t)a.splits * a.B * a.M * a.Hkv * (2 * a.d + a.dv_w) * sizeof(float);
+}
+size_t delta_bytes(const Args& a) { return ((size_t)a.B * a.H * 3 * a.N * sizeof(float) + 255) / 256 * 256; }
 
 int done(int rc, const char* what) {
   if (rc == -3) return fail("%s: too many tokens for one launch", what);
@@ -112,7 +124,9 @@ extern "C" size_t scgg_diff_attention_forward_workspace_bytes(const scgg_diff_at
 
 extern "C" size_t scgg_diff_attention_backward_workspace_bytes(const scgg_diff_attention_args* p) {
   if (check(p, "diff_attention_backward_workspace_bytes")) return 0;
-  return delta_bytes(make(p));
+  Args a = make(p);
+  plan_dkv(a);
+  return delta_bytes(a) + dkv_part_bytes(a);
 }
 
 extern "C" int scgg_diff_attention_forward(const scgg_diff_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -141,9 +155,11 @@ extern "C" int scgg_diff_attention_backward(const scgg_diff_attention_args* p, v
     return fail("%s: base and strides of dout have to be multiples of 16 bytes", what);
   if (queries && !near(p, p->dout_stride_n, 0, p->dv)) return fail("%s: rows of dout have to lie less than 2 GiB / 64 apart", what);
   Args a = make(p);
-  const size_t need = delta_bytes(a);
+  plan_dkv(a);
+  const size_t need = delta_bytes(a) + dkv_part_bytes(a);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
   a.delta = static_cast<float*>(workspace);
+  a.part = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int rc = p->dtype == SCGG_F32 ? run_backward<float>(a, st) : p->dtype == SCGG_BF16 ? run_backward<__bf16>(a, st) : run_backward<_Float16>(a, st);
   if (rc == 0) hipLaunchKernelGGL(dlambda_kernel, dim3((unsigned)p->H), dim3(256), 0, st, a.delta, p->dlambda, p->B, p->H, p->N);

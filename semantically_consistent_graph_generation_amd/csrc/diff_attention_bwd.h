@@ -75,13 +75,13 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   auto score = [&](int i, int hh) {
     Dot<T> s;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh, i * (DP / 16) + c, lane), qf[i][c]);
     return s.sum();
   };
   auto dprob = [&](int hh) {
     Dot<T> s;
 #pragma unroll
-    for (int c = 0; c < DVP / 16; ++c) s.add(VTile::rows(vt, 32 * hh + l31, 2 * c + g), gf[c]);
+    for (int c = 0; c < DVP / 16; ++c) s.add(VTile::rows(vt, 32 * hh, c, lane), gf[c]);
     return s.sum();
   };
   auto seen = [&](int t, u64 bits) { return a.causal ? bits & upto(q + off - (long long)t * TILE) : bits; };
@@ -231,40 +231,55 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
 template <class T, int DP, int DVP>
 struct DkvShape {
   static constexpr int P = Type<T>::planes, ND = (DP + 31) / 32, NV = DVP / 32;
-  typedef Tile<2 * DP, P> QTile;
-  typedef Tile<DVP, P> GTile;
-  static constexpr int TILES = QTile::BYTES + GTile::BYTES;
-  static constexpr int MERGE = 2 * (2 * ND + NV) * 16 * 64 * 4;
-  static constexpr int ROWS = TILES > MERGE ? TILES : MERGE;      // offset of the rows' statistics [6][TILE]
-  static constexpr int LDS = ROWS + 6 * TILE * 4;
-  static constexpr int MIN_BLOCKS = P == 1 && DP <= 32 ? 2 : 1;
+  // d > 32: the sums and operands of both gradients are more than half the registers of a SIMD, and one wave alone waits for each of its
+  // products; dK and dV then have a kernel each (the maps are formed twice), and their tiles are 32 queries, which halves what is under way
+  static constexpr bool APART = DP > 32;
+  static constexpr int MIN_BLOCKS = P == 1 ? 2 : 1, TQ = APART ? 32 : 64;
+  typedef Tile<2 * DP, P, TQ> QTile;
+  typedef Tile<DVP, P, TQ> GTile;
+  static constexpr int ROWS = QTile::BYTES + GTile::BYTES;          // offset of the rows' statistics [6][TQ]
+  static constexpr int LDS = ROWS + 6 * TQ * 4;
 };
+constexpr int BK = 128;                                             // keys of a workgroup: 32 per wave
 
 // Over keys: a wave keeps 32 of them (k1, k2 and v as operands, dK1, dK2 and dV as sums) and the queries of all heads that share the key
-// head stream by.  4 / QW groups of 32 keys, QW waves that share a tile's queries.
-template <class T, int DP, int DVP, int QW>
+// head stream by.  With few keys the queries are split over `splits` workgroups, whose sums go to `part` [splits][B M Hkv][2 d + dv]
+// in 32 bits and are added in order by dkv_join.  WHAT: 1 dK, 2 dV, 3 both.
+template <class T, int DP, int DVP, int WHAT>
 __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void dkv_kernel(Args a) {
+  constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   typedef DkvShape<T, DP, DVP> S;
   typedef typename S::QTile QTile;
   typedef typename S::GTile GTile;
-  constexpr int P = S::P, KG = 4 / QW, BK = 32 * KG, ND = S::ND, NV = S::NV;
+  constexpr int P = S::P, TQ = S::TQ, ND = S::ND, NV = S::NV;
   extern __shared__ __align__(256) char lds[];
   char* qt = lds;
   char* gt = lds + QTile::BYTES;
   float* rowst = reinterpret_cast<float*>(lds + S::ROWS);          // of the tile's queries: m and il of both maps (Prob), - w_i delta_i
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
-  const int kg = wave / QW, qw = wave - kg * QW;
-  const int k_tiles = (a.M + BK - 1) / BK, group = a.H / a.Hkv;
-  const unsigned id = die_major(blockIdx.x, gridDim.x);
-  const int bk = id / k_tiles, kt = id - bk * k_tiles, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-  const int key = kt * BK + 32 * kg + l31;
+  const int k_tiles = (a.M + BK - 1) / BK, group = a.H / a.Hkv, heads = a.B * a.Hkv;
+  int bk, kt, split;
+  if (a.causal) {                                                   // long ones first, over all dies
+    split = blockIdx.x % a.splits;
+    const int rest = blockIdx.x / a.splits;
+    kt = rest / heads;
+    bk = rest - kt * heads;
+  } else {
+    const unsigned id = die_major(blockIdx.x, gridDim.x);
+    split = id % a.splits;
+    const int rest = id / a.splits;
+    bk = rest / k_tiles;
+    kt = rest - bk * k_tiles;
+  }
+  const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int key = kt * BK + 32 * wave + l31;
   const bool k_in = key < a.M, k_on = k_in && (a.mask == nullptr || a.mask[b * a.mb + key] != 0);
   const long long off = (long long)a.M - a.N;                      // causal: key j is seen by the queries >= j - off
   Frag<P> kf[2][DP / 16], vf[DVP / 16];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     load_rows<T, DP>(kf[i], static_cast<const T*>(a.k) + b * a.kb + (long long)key * a.kn + (2ll * hk + i) * a.kh, k_on, a.d, g);
-  load_rows<T, DVP>(vf, static_cast<const T*>(a.v) + b * a.vb + (long long)key * a.vn + (long long)hk * a.vh, k_on, a.dv_w, g);
+  if (DK) load_rows<T, DVP>(vf, static_cast<const T*>(a.v) + b * a.vb + (long long)key * a.vn + (long long)hk * a.vh, k_on, a.dv_w, g);
 
   f32x16 dk[2][ND], dv[NV];
 #pragma unroll
@@ -290,164 +305,176 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
     up_s = pow2_below(16384.f, 2.f * lam * top);
   }
 
-  const int n_tiles = (a.N + TILE - 1) / TILE;
+  const int n_tiles = (a.N + TQ - 1) / TQ;
   int t_first = 0;
   if (a.causal) {
     const long long q_first = (long long)kt * BK - off;
-    if (q_first > 0) t_first = q_first / TILE < n_tiles ? (int)(q_first / TILE) : n_tiles;
+    if (q_first > 0) t_first = q_first / TQ < n_tiles ? (int)(q_first / TQ) : n_tiles;
   }
   // a workgroup whose keys are all hidden has nothing to sum
   const bool any = __syncthreads_or(k_on);
-  Stage<T, 2 * DP, 2> qs;
-  Stage<T, DVP, 1> gs;
+  Stage<T, 2 * DP, 2, TQ> qs;
+  Stage<T, DVP, 1, TQ> gs;
   qs.init(a.qn, a.qh, a.d, tid);
   gs.init(a.gn, 0, a.dv_w, tid);
   float2 rs;
   float rlam;
   auto load = [&](int hg, int t) {
     const int h = hk * group + hg;
-    const long long left = (long long)a.N - (long long)t * TILE;
-    const u64 bits = left >= TILE ? ~0ull : (1ull << left) - 1;
+    const long long left = (long long)a.N - (long long)t * TQ;
+    const u64 bits = left >= TQ ? ~0ull : (1ull << left) - 1;
     const long long bh = (long long)b * a.H + h;
-    const int n = t * TILE + lane;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
+    const int n = t * TQ + lane % TQ;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
     rlam = a.lambda[h];
     rs = wave < 2 ? make_float2(INFINITY, 0.f) : make_float2(0.f, 0.f);
     if (n < a.N) {
       if (wave < 2) rs = a.stats[(bh * 2 + wave) * a.N + n];
       else if (wave == 2) rs = make_float2(a.delta[bh * 3 * a.N + n], a.delta[(bh * 3 + 1) * a.N + n]);
     }
-    qs.load(static_cast<const T*>(a.q) + b * a.qb + 2ll * h * a.qh + (long long)t * TILE * a.qn, bits, tid);
-    gs.load(static_cast<const T*>(a.dout) + b * a.gb + (long long)h * a.gh + (long long)t * TILE * a.gn, bits, tid);
+    qs.load(static_cast<const T*>(a.q) + b * a.qb + 2ll * h * a.qh + (long long)t * TQ * a.qn, bits, tid);
+    gs.load(static_cast<const T*>(a.dout) + b * a.gb + (long long)h * a.gh + (long long)t * TQ * a.gn, bits, tid);
   };
-  int hg = 0, t = t_first;
-  const bool work = any && t_first < n_tiles;
-  if (work) load(hg, t);
-  while (work && hg < group) {
+  const long long per_head = n_tiles - t_first, steps = per_head * group;
+  long long step = steps * split / a.splits;
+  const long long last_step = any ? steps * (split + 1) / a.splits : step;
+  int hg = per_head > 0 ? (int)(step / per_head) : 0, t = t_first + (int)(step - hg * per_head);
+  if (step < last_step) load(hg, t);
+  for (; step < last_step; ++step) {
     __syncthreads();
     qs.put(qt, tid);
     gs.put(gt, tid);
     const float lam = rlam, w1 = up_s, w2 = -lam * up_s;
     if (wave < 2) {
       const Prob<T> pr(rs.x, rs.y, 1.f);
-      rowst[2 * wave * TILE + lane] = pr.m;
-      if (!Prob<T>::folded) rowst[(2 * wave + 1) * TILE + lane] = pr.f;
+      rowst[2 * wave * TQ + lane % TQ] = pr.m;
+      if (!Prob<T>::folded) rowst[(2 * wave + 1) * TQ + lane % TQ] = pr.f;
     } else if (wave == 2) {
-      rowst[4 * TILE + lane] = -w1 * rs.x;
-      rowst[5 * TILE + lane] = -w2 * rs.y;
+      rowst[4 * TQ + lane % TQ] = -w1 * rs.x;
+      rowst[5 * TQ + lane % TQ] = -w2 * rs.y;
     }
     __syncthreads();
     int t_next = t + 1, hg_next = hg;
     if (t_next == n_tiles) { t_next = t_first; ++hg_next; }
-    if (hg_next < group) load(hg_next, t_next);
+    if (step + 1 < last_step) load(hg_next, t_next);
 #pragma unroll
-    for (int half = 0; half < 2 / QW; ++half) {
-      const int hh = QW == 1 ? half : qw;
-      const long long last_q = (long long)t * TILE + 32 * hh + 31;
-      if (a.causal && last_q + off < (long long)kt * BK + 32 * kg) continue;   // no query of these sees a key of the wave
+    for (int hh = 0; hh < TQ / 32; ++hh) {
+      const long long last_q = (long long)t * TQ + 32 * hh + 31;
+      if (a.causal && last_q + off < (long long)kt * BK + 32 * wave) continue;   // no query of these sees a key of the wave
       auto score = [&](int i) {
         Dot<T> s;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) s.add(QTile::rows(qt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), kf[i][c]);
+        for (int c = 0; c < DP / 16; ++c) s.add(QTile::rows(qt, 32 * hh, i * (DP / 16) + c, lane), kf[i][c]);
         return s.sum();
       };
-      f32x16 s1 = score(0), s2 = score(1);
-      Dot<T> dot;
+      f32x16 dp;
+      if (DK) {
+        Dot<T> dot;
 #pragma unroll
-      for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh + l31, 2 * c + g), vf[c]);
-      const f32x16 dp = dot.sum();
-      if (a.causal && (long long)t * TILE + 32 * hh + off < (long long)kt * BK + 32 * kg + 31) {   // some query of these does not see some key
-        const long long from = key - off - (long long)t * TILE - 32 * hh;                             // the first that sees the lane's
-        const int first = from < 0 ? 0 : from > 32 ? 32 : (int)from;
+        for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh, c, lane), vf[c]);
+        dp = dot.sum();
+      }
+      const bool cut = a.causal && (long long)t * TQ + 32 * hh + off < (long long)kt * BK + 32 * wave + 31;   // some query does not see some key
+      const long long from = cut ? key - off - (long long)t * TQ - 32 * hh : 0;                          // the first that sees the lane's
+      const int first = from < 0 ? 0 : from > 32 ? 32 : (int)from;
+      Frag<P> fa[2], fs[2][2];
+      float p[16];                                                  // P1, then A
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool on = 8 * (r >> 2) + 4 * g + (r & 3) >= first;
-          s1[r] = on ? s1[r] : -INFINITY;
-          s2[r] = on ? s2[r] : -INFINITY;
+      for (int i = 0; i < 2; ++i) {
+        f32x16 s = score(i);
+        if (cut) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + 4 * g + (r & 3) >= first ? s[r] : -INFINITY;
+        }
+        float ds[16];
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int row = 32 * hh + 8 * r4 + 4 * g;
+          const f32x4 m = *reinterpret_cast<const f32x4*>(rowst + 2 * i * TQ + row), e = *reinterpret_cast<const f32x4*>(rowst + (4 + i) * TQ + row);
+          f32x4 il = {1.f, 1.f, 1.f, 1.f};
+          if (!Prob<T>::folded) il = *reinterpret_cast<const f32x4*>(rowst + (2 * i + 1) * TQ + row);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = 4 * r4 + x;
+            float q = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -m[x]));
+            if (!Prob<T>::folded) q *= il[x];
+            if (DK) ds[r] = q * fmaf(dp[r], i == 0 ? w1 : w2, e[x]);
+            p[r] = i == 0 ? q : fmaf(-lam, q, p[r]) * up_a;
+          }
+        }
+        if (DK) {
+          fs[i][0] = pack8<T>(ds);
+          fs[i][1] = pack8<T>(ds + 8);
         }
       }
-      float pa[16], d1[16], d2[16];
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int row = 32 * hh + 8 * r4 + 4 * g;
-        const f32x4 m1 = *reinterpret_cast<const f32x4*>(rowst + row), m2 = *reinterpret_cast<const f32x4*>(rowst + 2 * TILE + row),
-                    e1 = *reinterpret_cast<const f32x4*>(rowst + 4 * TILE + row), e2 = *reinterpret_cast<const f32x4*>(rowst + 5 * TILE + row);
-        f32x4 i1, i2;
-        if (!Prob<T>::folded) {
-          i1 = *reinterpret_cast<const f32x4*>(rowst + TILE + row);
-          i2 = *reinterpret_cast<const f32x4*>(rowst + 3 * TILE + row);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = 4 * r4 + x;
-          float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -m1[x])), p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -m2[x]));
-          if (!Prob<T>::folded) { p1 *= i1[x]; p2 *= i2[x]; }
-          pa[r] = fmaf(-lam, p2, p1) * up_a;
-          d1[r] = p1 * fmaf(dp[r], w1, e1[x]);
-          d2[r] = p2 * fmaf(dp[r], w2, e2[x]);
-        }
+      if (DV) {
+        fa[0] = pack8<T>(p);
+        fa[1] = pack8<T>(p + 8);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int row0 = 32 * hh + 16 * u;
-        const Frag<P> fa = pack8<T>(pa + 8 * u), f1 = pack8<T>(d1 + 8 * u), f2 = pack8<T>(d2 + 8 * u);
+        if (DV) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) accumulate<T>(dv[j], GTile::cols(gt, row0, 32 * j, lane, DVP), fa);
+          for (int j = 0; j < NV; ++j) accumulate<T>(dv[j], GTile::cols(gt, row0, 32 * j, lane, DVP), fa[u]);
+        }
+        if (DK) {
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          accumulate<T>(dk[0][j], QTile::cols(qt, row0, 32 * j, lane, DP), f1);
-          accumulate<T>(dk[1][j], QTile::cols(qt, row0, DP + 32 * j, lane, 2 * DP), f2);
+          for (int j = 0; j < ND; ++j) {
+            accumulate<T>(dk[0][j], QTile::cols(qt, row0, 32 * j, lane, DP), fs[0][u]);
+            accumulate<T>(dk[1][j], QTile::cols(qt, row0, DP + 32 * j, lane, 2 * DP), fs[1][u]);
+          }
         }
       }
     }
     t = t_next;
     hg = hg_next;
   }
-  if constexpr (QW == 2) {
-    float* box = reinterpret_cast<float*>(lds) + (size_t)kg * (2 * ND + NV) * 16 * 64;
-    __syncthreads();
-    if (qw == 1) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) box[(j * 16 + r) * 64 + lane] = dv[j][r];
-#pragma unroll
-      for (int j = 0; j < 2 * ND; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) box[((NV + j) * 16 + r) * 64 + lane] = dk[j / ND][j % ND][r];
-    }
-    __syncthreads();
-    if (qw == 1) return;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dv[j][r] += box[(j * 16 + r) * 64 + lane];
-#pragma unroll
-    for (int j = 0; j < 2 * ND; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dk[j / ND][j % ND][r] += box[((NV + j) * 16 + r) * 64 + lane];
-  }
   if (!k_in) return;
   const float fv = k_on ? 1.f / up_a : 0.f, fk = k_on ? a.scale / up_s : 0.f;
   auto out = [&](float x, float f) { return k_on ? x * f : 0.f; };   // a hidden key's sums may hold anything
-  T* dst = static_cast<T*>(a.dv) + (((long long)b * a.M + key) * a.Hkv + hk) * a.dv_w;
+  const long long row = ((long long)b * a.M + key) * a.Hkv + hk;
+  float* part = a.splits > 1 ? a.part + ((long long)split * a.B * a.M * a.Hkv + row) * (2 * a.d + a.dv_w) : nullptr;
+  auto put = [&](T* dst, float* to, const f32x16& v, int r, float f) {
+    if (part != nullptr) *reinterpret_cast<f32x4*>(to) = f32x4{out(v[r], f), out(v[r + 1], f), out(v[r + 2], f), out(v[r + 3], f)};
+    else store4<T>(dst, out(v[r], f), out(v[r + 1], f), out(v[r + 2], f), out(v[r + 3], f));
+  };
+  if (DV) {
+    T* dst = static_cast<T*>(a.dv) + row * a.dv_w;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int col = 32 * j + 2 * r + 4 * g;
-      if (col < a.dv_w) store4<T>(dst + col, out(dv[j][r], fv), out(dv[j][r + 1], fv), out(dv[j][r + 2], fv), out(dv[j][r + 3], fv));
-    }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    T* kd = static_cast<T*>(a.dk) + (((long long)b * a.M + key) * 2 * a.Hkv + 2 * hk + i) * a.d;
-#pragma unroll
-    for (int j = 0; j < ND; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int col = 32 * j + 2 * r + 4 * g;
-        if (col < a.d) store4<T>(kd + col, out(dk[i][j][r], fk), out(dk[i][j][r + 1], fk), out(dk[i][j][r + 2], fk), out(dk[i][j][r + 3], fk));
+        if (col < a.dv_w) put(dst + col, part + 2 * a.d + col, dv[j], r, fv);
       }
   }
+  if (DK) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      T* dst = static_cast<T*>(a.dk) + (row * 2 + i) * a.d;
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int col = 32 * j + 2 * r + 4 * g;
+          if (col < a.d) put(dst + col, part + i * a.d + col, dk[i][j], r, fk);
+        }
+    }
+  }
+}
+
+// the splits' sums of four neighbouring columns, in order
+template <class T>
+__global__ __launch_bounds__(256) void dkv_join(Args a, long long quads) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  const int width = 2 * a.d + a.dv_w;
+  const long long row = i / (width / 4);
+  const int col = (int)(i - row * (width / 4)) * 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.part + s * quads * 4 + i * 4);
+  T* dst = col < 2 * a.d ? static_cast<T*>(a.dk) + row * 2 * a.d + col : static_cast<T*>(a.dv) + row * a.dv_w + (col - 2 * a.d);
+  store4<T>(dst, v[0], v[1], v[2], v[3]);
 }
 
 template <class T, int DP, int DVP, int KW>
@@ -461,22 +488,33 @@ int launch_dq(const Args& a, hipStream_t st) {
   return 0;
 }
 
-template <class T, int DP, int DVP, int QW>
+template <class T, int DP, int DVP, int WHAT>
 int launch_dkv(const Args& a, hipStream_t st) {
   typedef DkvShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, QW>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.Hkv * ((a.M + 128 / QW - 1) / (128 / QW));
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT>), S::LDS)) return -2;
+  const long long blocks = (long long)a.B * a.Hkv * ((a.M + BK - 1) / BK) * a.splits;
   if (blocks > 0x7fffffffLL) return -3;
-  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, QW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
 
 template <class T, int DP, int DVP>
 int launch_bwd(const Args& a, hipStream_t st) {
-  const bool few_q = (long long)a.B * a.H * ((a.N + 127) / 128) < 512, few_k = (long long)a.B * a.Hkv * ((a.M + 127) / 128) < 256;
+  const bool few_q = (long long)a.B * a.H * ((a.N + 127) / 128) < 512;
   if (const int rc = few_q ? launch_dq<T, DP, DVP, 2>(a, st) : launch_dq<T, DP, DVP, 1>(a, st)) return rc;
-  return few_k ? launch_dkv<T, DP, DVP, 2>(a, st) : launch_dkv<T, DP, DVP, 1>(a, st);
+  if constexpr (DkvShape<T, DP, DVP>::APART) {
+    if (const int rc = launch_dkv<T, DP, DVP, 1>(a, st)) return rc;
+    if (const int rc = launch_dkv<T, DP, DVP, 2>(a, st)) return rc;
+  } else {
+    if (const int rc = launch_dkv<T, DP, DVP, 3>(a, st)) return rc;
+  }
+  const long long quads = (long long)a.B * a.M * a.Hkv * (2 * a.d + a.dv_w) / 4;
+  if (a.splits > 1 && quads > 0) {
+    if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
+    hipLaunchKernelGGL((dkv_join<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, quads);
+  }
+  return 0;
 }
 
 template <class T>

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
   auto score = [&](int i, int hh) {
     Dot<T> s;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+    for (int c = 0; c < DP / 16; ++c) s.add(KTile::rows(kt, 32 * hh, i * (DP / 16) + c, lane), qf[i][c]);
     return s.sum();
   };
   auto seen = [&](int t, u64 bits) { return a.causal ? bits & upto(q + off - (long long)t * TILE) : bits; };
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
     for (int i = 0; i < 2; ++i) {
       Dot<T> dot;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) dot.add(KTile::rows(kt, 32 * hh + l31, i * (DP / 8) + 2 * c + g), qf[i][c]);
+      for (int c = 0; c < DP / 16; ++c) dot.add(KTile::rows(kt, 32 * hh, i * (DP / 16) + c, lane), qf[i][c]);
       f32x16 s = dot.sum();
       if (part) hide(s, see, hh, g);
       float top = row_max(s) * a.c;
