@@ -238,7 +238,11 @@ struct DkvShape {
   typedef Tile<2 * DP, P, TQ> QTile;
   typedef Tile<DVP, P, TQ> GTile;
   static constexpr int ROWS = QTile::BYTES + GTile::BYTES;          // offset of the rows' statistics [6][TQ]
-  static constexpr int LDS = ROWS + 6 * TQ * 4;
+  static constexpr int KEYS = ROWS + 6 * TQ * 4;                    // offset of v, where it is kept in LDS
+  typedef Tile<DVP, P, 128> VTile;
+  // dK at d > 32 in 16 bits: with v in registers too a few of them would go to memory, and every such access waits for the next tile's loads
+  static constexpr bool V_LDS = APART && P == 1;
+  static constexpr int lds(int what) { return KEYS + (V_LDS && what == 1 ? VTile::BYTES : 0); }
 };
 constexpr int BK = 128;                                             // keys of a workgroup: 32 per wave
 
@@ -275,11 +279,25 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
   const int key = kt * BK + 32 * wave + l31;
   const bool k_in = key < a.M, k_on = k_in && (a.mask == nullptr || a.mask[b * a.mb + key] != 0);
   const long long off = (long long)a.M - a.N;                      // causal: key j is seen by the queries >= j - off
-  Frag<P> kf[2][DP / 16], vf[DVP / 16];
+  constexpr bool V_LDS = S::V_LDS && WHAT == 1;
+  char* vt = lds + S::KEYS;
+  Frag<P> kf[2][DP / 16], vf[V_LDS ? 1 : DVP / 16];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     load_rows<T, DP>(kf[i], static_cast<const T*>(a.k) + b * a.kb + (long long)key * a.kn + (2ll * hk + i) * a.kh, k_on, a.d, g);
-  if (DK) load_rows<T, DVP>(vf, static_cast<const T*>(a.v) + b * a.vb + (long long)key * a.vn + (long long)hk * a.vh, k_on, a.dv_w, g);
+  const T* v_row = static_cast<const T*>(a.v) + b * a.vb + (long long)key * a.vn + (long long)hk * a.vh;
+  if constexpr (V_LDS) {                                           // a wave reads its own rows only
+#pragma unroll
+    for (int c = 0; c < DVP / 16; ++c) {
+      Raw<T> r;
+      const int col = 16 * c + 8 * g;
+      if (k_on && col < a.dv_w) r.load(v_row + col);
+      else r.clear();
+      S::VTile::put(vt, 32 * wave + l31, 2 * c + g, r.frag());
+    }
+  } else if constexpr (DK) {
+    load_rows<T, DVP>(vf, v_row, k_on, a.dv_w, g);
+  }
 
   f32x16 dk[2][ND], dv[NV];
 #pragma unroll
@@ -370,7 +388,7 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
       if (DK) {
         Dot<T> dot;
 #pragma unroll
-        for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh, c, lane), vf[c]);
+        for (int c = 0; c < DVP / 16; ++c) dot.add(GTile::rows(gt, 32 * hh, c, lane), V_LDS ? S::VTile::rows(vt, 32 * wave, c, lane) : vf[V_LDS ? 0 : c]);
         dp = dot.sum();
       }
       const bool cut = a.causal && (long long)t * TQ + 32 * hh + off < (long long)kt * BK + 32 * wave + 31;   // some query does not see some key
@@ -492,10 +510,10 @@ template <class T, int DP, int DVP, int WHAT>
 int launch_dkv(const Args& a, hipStream_t st) {
   typedef DkvShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT>), S::LDS)) return -2;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT>), S::lds(WHAT))) return -2;
   const long long blocks = (long long)a.B * a.Hkv * ((a.M + BK - 1) / BK) * a.splits;
   if (blocks > 0x7fffffffLL) return -3;
-  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT>), dim3((unsigned)blocks), dim3(THREADS), S::lds(WHAT), st, a);
   return 0;
 }
 
