@@ -39,9 +39,10 @@ def _check_heads(what, name, t, like=None):
         _fail(what, f"{name} has to be a tensor")
     if t.dim() != 4:
         _fail(what, f"{name} has to be [B, tokens, heads, width], got {tuple(t.shape)}")
-    if t.dtype not in _DTYPES:
-        _fail(what, f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is None:
+        if t.dtype not in _DTYPES:
+            _fail(what, f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")
+    elif t.dtype != like.dtype or t.device != like.device:
         _fail(what, f"{name} is {t.dtype} on {t.device}, q is {like.dtype} on {like.device}")
 
 
@@ -68,9 +69,18 @@ def _aligned_rows(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+# the stream's handle without a Stream object around it, where this torch has it: 2 us of a call's 15
+_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _new(t):
+    """A contiguous tensor like t, not filled."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _call(device, fn, *args):
     """``fn(*args, stream)`` with the tensors' device current, on its current stream."""
-    stream = C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    stream = _stream_handle(device.index)
     if torch.cuda.current_device() == device.index:
         return fn(*args, stream)
     with torch.cuda.device(device):
@@ -116,7 +126,7 @@ def _rope_forward(q, k, wq, wk, pos, cfg):
         if t is None:
             out.append(None)
             continue
-        y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        y = _new(t)
         _rope_set(a, "x", i, t)
         a.y[i] = y.data_ptr()
         out.append(y)
@@ -144,7 +154,7 @@ class _Rope(torch.autograd.Function):
         for i, g in enumerate(gs):
             if g is None:
                 continue
-            grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+            grads[i] = _new(g)
             _rope_set(a, "g", i, g)
             a.y[i] = grads[i].data_ptr()
             if ctx.norm:
@@ -283,7 +293,7 @@ class _DiffAttention(torch.autograd.Function):
         a = _diff_args(q, k, v, lam, mask, ctx.cfg)
         dout = _aligned_rows(dout)
         _diff_set(a, "dout", dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = _new(q), _new(k), _new(v)
         dlam = torch.empty_like(lam)
         a.stats, a.dq, a.dk, a.dv_out, a.dlambda = stats.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr()
         nbytes = L.scgg_diff_attention_backward_workspace_bytes(C.byref(a))

@@ -255,10 +255,8 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
   const int hh = wave & 1, vw = wave >> 1;
   const int group = a.H / a.Hkv, rows = a.N * group, blocks = (rows + 31) / 32;
-  unsigned id = blockIdx.x;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int rb = id % blocks, bk = id / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int at = blockIdx.x / a.splits, rb = at % blocks, bk = at / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int split = (int)((blockIdx.x + bk) % a.splits);       // turned by the head: the dies (ids modulo 8) share the ends of short sequences
   const int row = rb * 32 + l31, n = row / group, h = hk * group + (row - n * group);
   const bool on = row < rows;
   const long long off = (long long)a.M - a.N;
@@ -323,10 +321,12 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
         sum += p[r];
       }
       l[i] = l[i] * keep + sum;
+      if (__any(keep != 1.f)) {                                    // most tiles leave every maximum as it is
 #pragma unroll
-      for (int j = 0; j < NW; ++j)
+        for (int j = 0; j < NW; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][j][r] *= keep;
+          for (int r = 0; r < 16; ++r) o[i][j][r] *= keep;
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const Frag<P> pf = pack8<T>(p + 8 * u);
@@ -370,36 +370,50 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   }
 }
 
-// one workgroup of 64 per (sequence, query, head): the parts of a row, in order
+// One workgroup per (sequence, query, head): the parts of a row.  A wave holds every part's weight (one lane a part, 64 at a time); the four
+// waves each take every fourth part, and their sums are added in order.
 template <class T>
-__global__ __launch_bounds__(64) void split_join(Args a) {
-  const int id = blockIdx.x, h = id % a.H, bn = id / a.H, n = bn % a.N, b = bn / a.N, lane = threadIdx.x;
+__global__ __launch_bounds__(THREADS) void split_join(Args a) {
+  __shared__ float w1[64], w2[64];
+  __shared__ f32x4 sum[4][32];
+  const int id = blockIdx.x, h = id % a.H, bn = id / a.H, n = bn % a.N, b = bn / a.N, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int group = a.H / a.Hkv, hk = h / group, rows = a.N * group, row = n * group + (h - hk * group);
   const int slots = 2 * a.splits, ld = 2 * a.dv_w + 4;
   const float* in = a.part + ((long long)(b * a.Hkv + hk) * rows + row) * slots * ld;
-  float w[2], mc[2], il[2];
+  float w[2], mc[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float m = -INFINITY, l = 0.f;
     for (int s = lane; s < slots; s += 64) merge_stats(m, l, in[s * ld + 2 * a.dv_w + 2 * i], in[s * ld + 2 * a.dv_w + 2 * i + 1]);
     for (int x = 1; x < 64; x <<= 1) merge_stats(m, l, __shfl_xor(m, x), __shfl_xor(l, x));
     mc[i] = l == 0.f ? INFINITY : m;
-    il[i] = l == 0.f ? 0.f : 1.f / l;
-    w[i] = i == 0 ? il[0] : -a.lambda[h] * il[1];
-    if (a.stats != nullptr && lane == 0) a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + n] = make_float2(mc[i], il[i]);
+    w[i] = l == 0.f ? 0.f : 1.f / l;
+    if (a.stats != nullptr && threadIdx.x == 0) a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + n] = make_float2(mc[i], w[i]);
   }
-  T* out = static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w;
-  for (int c = 4 * lane; c < a.dv_w; c += 256) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < slots; ++s) {
-      const float* p = in + (long long)s * ld;
-      const float e1 = w[0] * __builtin_amdgcn_exp2f(p[2 * a.dv_w] - mc[0]), e2 = w[1] * __builtin_amdgcn_exp2f(p[2 * a.dv_w + 2] - mc[1]);
-      const f32x4 o1 = *reinterpret_cast<const f32x4*>(p + c), o2 = *reinterpret_cast<const f32x4*>(p + a.dv_w + c);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += e1 * o1[r] + e2 * o2[r];
+  w[1] *= -a.lambda[h];
+  const int c = 4 * (lane & 31), side = lane >> 5;                 // lanes 0..31: P1 v, 32..63: P2 v; four columns each
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    __syncthreads();
+    if (threadIdx.x < 64 && s0 + lane < slots) {
+      const float* p = in + (long long)(s0 + lane) * ld + 2 * a.dv_w;
+      w1[lane] = w[0] * __builtin_amdgcn_exp2f(p[0] - mc[0]);
+      w2[lane] = w[1] * __builtin_amdgcn_exp2f(p[2] - mc[1]);
     }
-    store4<T>(out + c, v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    const int end = slots - s0 < 64 ? slots - s0 : 64;
+    if (c < a.dv_w) {
+#pragma unroll 4
+      for (int s = wave; s < end; s += 4) v += (side ? w2[s] : w1[s]) * *reinterpret_cast<const f32x4*>(in + (long long)(s0 + s) * ld + side * a.dv_w + c);
+    }
   }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] += __shfl_xor(v[r], 32);
+  if (side == 0) sum[wave][lane] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= a.dv_w) return;
+  v = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+  store4<T>(static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w + c, v[0], v[1], v[2], v[3]);
 }
 
 template <class T, int DP, int DVP, int KW>
@@ -421,7 +435,7 @@ int launch_split(const Args& a, hipStream_t st) {
   const long long rows = (long long)a.N * (a.H / a.Hkv), blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32) * a.splits;
   if (blocks > 0x7fffffffLL || (long long)a.B * a.N * a.H > 0x7fffffffLL) return -3;
   hipLaunchKernelGGL((split_kernel<T, DP, DVP>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
-  hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(64), 0, st, a);
+  hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(THREADS), 0, st, a);
   return 0;
 }
 
