@@ -240,32 +240,30 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
 }
 
 // A few rows against many keys: one pass over k and v, the keys split over workgroups.  The rows of a key head's group (queries x
-// heads that share it) are the columns of a 32-wide block.  The two key halves of a tile go to two waves each, which share the columns of v; every
-// such half keeps its own maximum, sum and (P v) of both maps, and `split_join` merges them.  P is at most 1 here and not yet A, so it is
-// taken in two terms (h + l): the pass waits for memory, the products are free.
+// heads that share it) are the columns of a 32-wide block.  A wave takes one map and one half of a tile's keys and keeps its own
+// maximum, sum and P v, which split_join merges.  P is at most 1 here and not yet A, so it is taken in two terms (h + l): the
+// pass waits for memory, the products are free.
 template <class T, int DP, int DVP>
 __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void split_kernel(Args a) {
   typedef FwdShape<T, DP, DVP> S;
   typedef typename S::KTile KTile;
   typedef typename S::VTile VTile;
-  constexpr int P = S::P, NV = DVP / 32, NW = (NV + 1) / 2;     // column tiles of v, per wave
+  constexpr int P = S::P, NV = DVP / 32;
   extern __shared__ __align__(256) char lds[];
   char* kt = lds;
   char* vt = lds + KTile::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
-  const int hh = wave & 1, vw = wave >> 1;
-  const int group = a.H / a.Hkv, rows = a.N * group, blocks = (rows + 31) / 32;
-  const int at = blockIdx.x / a.splits, rb = at % blocks, bk = at / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-  const int split = (int)((blockIdx.x + bk) % a.splits);       // turned by the head: the dies (ids modulo 8) share the ends of short sequences
-  const int row = rb * 32 + l31, n = row / group, h = hk * group + (row - n * group);
-  const bool on = row < rows;
+  const int hh = wave & 1, map = wave >> 1;
+  const int group = a.H / a.Hkv, rows = a.N * group;             // at most 32
+  const int bk = blockIdx.x / a.splits, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int split = (int)((blockIdx.x + bk) % a.splits);        // turned by the head: the dies (ids modulo 8) share the ends of short sequences
+  const int n = l31 / group, h = hk * group + (l31 - n * group);
+  const bool on = l31 < rows;
   const long long off = (long long)a.M - a.N;
   const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
   const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
-  Frag<P> qf[2][DP / 16];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)n * a.qn + (2ll * h + i) * a.qh, on, a.d, g);
+  Frag<P> qf[DP / 16];
+  load_rows<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qb + (long long)n * a.qn + (2ll * h + map) * a.qh, on, a.d, g);
 
   KeyBits keys;
   keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
@@ -278,12 +276,10 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   Stage<T, DVP, 1> vs;
   ks.init(a.kn, a.kh, a.d, tid);
   vs.init(a.vn, 0, a.dv_w, tid);
-  f32x16 o[2][NW];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  f32x16 o[NV];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < NW; ++j) o[i][j] = zero16();
+  for (int j = 0; j < NV; ++j) o[j] = zero16();
   u64 bits, bits_next;
   keys.start(first, wave, lane);
   int t = keys.next(first, bits, wave, lane);
@@ -302,72 +298,61 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
       vs.load(vp + (long long)tn * TILE * a.vn, bits_next, tid);
     }
     const u64 see = a.causal ? bits & upto(n + off - (long long)t * TILE) : bits;
-    const bool part = __any(see != ~0ull);
+    Dot<T> dot;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      Dot<T> dot;
+    for (int c = 0; c < DP / 16; ++c) dot.add(KTile::rows(kt, 32 * hh, map * (DP / 16) + c, lane), qf[c]);
+    f32x16 s = dot.sum();
+    if (__any(see != ~0ull)) hide(s, see, hh, g);
+    float top = row_max(s) * a.c;
+    top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);            // one maximum for both halves of the wave: they share a column of o
+    const float tc = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - tc);
+    m = top;
+    float p[16], sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) dot.add(KTile::rows(kt, 32 * hh, i * (DP / 16) + c, lane), qf[i][c]);
-      f32x16 s = dot.sum();
-      if (part) hide(s, see, hh, g);
-      float top = row_max(s) * a.c;
-      top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[i]);       // one maximum for both halves of the wave: they share a column of o
-      const float tc = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[i] - tc);
-      m[i] = top;
-      float p[16], sum = 0.f;
+    for (int r = 0; r < 16; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -tc));
+      sum += p[r];
+    }
+    l = fmaf(l, keep, sum);
+    if (__any(keep != 1.f)) {                                    // most tiles leave every maximum as it is
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -tc));
-        sum += p[r];
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[j][r] *= keep;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const Frag<P> pf = pack8<T>(p + 8 * u);
+      Frag<P> rest = pf;
+      if constexpr (P == 1) {
+        float q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = p[8 * u + j] - (float)(T)p[8 * u + j];
+        rest = pack8<T>(q);
       }
-      l[i] = l[i] * keep + sum;
-      if (__any(keep != 1.f)) {                                    // most tiles leave every maximum as it is
 #pragma unroll
-        for (int j = 0; j < NW; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][j][r] *= keep;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const Frag<P> pf = pack8<T>(p + 8 * u);
-        Frag<P> rest = pf;
-        if constexpr (P == 1) {
-          float q[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) q[j] = p[8 * u + j] - (float)(T)p[8 * u + j];
-          rest = pack8<T>(q);
-        }
-#pragma unroll
-        for (int j = 0; j < NW; ++j) {
-          const int col = 32 * (vw + 2 * j);
-          if (col < DVP) {
-            const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, col, lane, DVP);
-            if constexpr (P == 1) accumulate<T>(o[i][j], vf, rest);
-            accumulate<T>(o[i][j], vf, pf);
-          }
-        }
+      for (int j = 0; j < NV; ++j) {
+        const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, 32 * j, lane, DVP);
+        if constexpr (P == 1) accumulate<T>(o[j], vf, rest);
+        accumulate<T>(o[j], vf, pf);
       }
     }
     t = tn;
     bits = bits_next;
   }
   // part: [bk][row][2 splits + half][2 dv + 4]: o1, o2, m1, l1, m2, l2
-#pragma unroll
-  for (int i = 0; i < 2; ++i) l[i] += __shfl_xor(l[i], 32);
+  l += __shfl_xor(l, 32);
   if (!on) return;
   const int slots = 2 * a.splits, ld = 2 * a.dv_w + 4;
-  float* out = a.part + (((long long)bk * rows + row) * slots + 2 * split + hh) * ld;
+  float* out = a.part + (((long long)bk * rows + l31) * slots + 2 * split + hh) * ld;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int col = 32 * (vw + 2 * j) + 2 * r + 4 * g;
-        if (col < a.dv_w) *reinterpret_cast<f32x4*>(out + i * a.dv_w + col) = f32x4{o[i][j][r], o[i][j][r + 1], o[i][j][r + 2], o[i][j][r + 3]};
-      }
-    if (vw == 0 && g == 0) { out[2 * a.dv_w + 2 * i] = m[i]; out[2 * a.dv_w + 2 * i + 1] = l[i]; }
-  }
+    for (int r = 0; r < 16; r += 4) {
+      const int col = 32 * j + 2 * r + 4 * g;
+      if (col < a.dv_w) *reinterpret_cast<f32x4*>(out + map * a.dv_w + col) = f32x4{o[j][r], o[j][r + 1], o[j][r + 2], o[j][r + 3]};
+    }
+  if (g == 0) { out[2 * a.dv_w + 2 * map] = m; out[2 * a.dv_w + 2 * map + 1] = l; }
 }
 
 // One workgroup per (sequence, query, head): the parts of a row.  A wave holds every part's weight (one lane a part, 64 at a time); the four
@@ -432,7 +417,7 @@ int launch_split(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&split_kernel<T, DP, DVP>), S::LDS)) return -2;
-  const long long rows = (long long)a.N * (a.H / a.Hkv), blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32) * a.splits;
+  const long long blocks = (long long)a.B * a.Hkv * a.splits;
   if (blocks > 0x7fffffffLL || (long long)a.B * a.N * a.H > 0x7fffffffLL) return -3;
   hipLaunchKernelGGL((split_kernel<T, DP, DVP>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(THREADS), 0, st, a);
