@@ -62,3 +62,41 @@ def diff_attention(q, k, v, lam, key_mask=None, causal=False, scale=None):
     p1, p2 = softmax_maps(q, k, see, q.shape[-1] ** -0.5 if scale is None else scale)
     v = v.repeat_interleave(p1.shape[1] // v.shape[2], 2)
     return torch.einsum("bhnm,bmhe->bnhe", p1 - lam[None, :, None, None] * p2, v)
+
+
+def sit_differential(sd, x, t, mask, n_blocks, n_heads, theta=100.0):
+    """The node-coordinate transformer with differential attention (node_coordinate_diffusion.SiT(attention="differential")) on a
+    plain state_dict, in the type of its tensors (float64 in the tests)."""
+    import math
+    import torch.nn.functional as F
+
+    def lin(name, v):
+        return F.linear(v, sd[name + ".weight"], sd[name + ".bias"])
+
+    def ln(v):
+        return F.layer_norm(v, (v.shape[-1],), eps=1e-6)
+    h = lin("pos_embedder", x)
+    B, N, dim = h.shape
+    half = sd["t_embedder.mlp.0.weight"].shape[1] // 2
+    arg = t.to(x)[:, None] * torch.exp(torch.arange(half).to(x) * (-math.log(10000.0) / half))
+    c = lin("t_embedder.mlp.2", F.silu(lin("t_embedder.mlp.0", torch.cat([arg.cos(), arg.sin()], -1))))
+    d, H = dim // n_heads, n_heads // 2
+    axes, pairs = x.shape[-1], d // 2
+    sections = [pairs // axes + (1 if a < pairs % axes else 0) for a in range(axes)]
+    for i in range(n_blocks):
+        p = f"blocks.{i}."
+        a = p + "attn."
+        sh1, sc1, g1, sh2, sc2, g2 = lin(p + "adaLN_modulation.1", F.silu(c)).chunk(6, 1)
+        qkv = lin(a + "qkv", ln(h) * (1 + sc1[:, None]) + sh1[:, None])
+        q, k = (qkv[..., j * dim:(j + 1) * dim].reshape(B, N, 2 * H, d) for j in (0, 1))
+        v = qkv[..., 2 * dim:].reshape(B, N, H, 2 * d)
+        q = qk_norm_rope(q, sd[a + "q_norm"], x.detach(), sections, theta)
+        k = qk_norm_rope(k, sd[a + "k_norm"], x.detach(), sections, theta)
+        start = 0.8 - 0.6 * math.exp(-0.3 * i)
+        lam = (sd[a + "lambda_q1"] @ sd[a + "lambda_k1"]).exp() - (sd[a + "lambda_q2"] @ sd[a + "lambda_k2"]).exp() + start
+        o = head_norm(diff_attention(q, k, v, lam.expand(H), key_mask=mask), sd[a + "out_norm"]) * (1 - start)
+        h = h + g1[:, None] * lin(a + "proj", o.reshape(B, N, dim))
+        u = ln(h) * (1 + sc2[:, None]) + sh2[:, None]
+        h = h + g2[:, None] * lin(p + "mlp.fc2", F.gelu(lin(p + "mlp.fc1", u), approximate="tanh"))
+    sh, sc = lin("final_layer.adaLN_modulation.1", F.silu(c)).chunk(2, 1)
+    return lin("final_layer.linear", ln(h) * (1 + sc[:, None]) + sh[:, None]) * mask[..., None]

@@ -8,21 +8,53 @@ The arithmetic runs in libscgg.so (``scgg_sit_forward`` / ``scgg_sit_sample``, c
 The reference's checkpoints (``cow_best_coord_model.pth``) are not in its repository: weights are whatever the caller loads.
 Parity: the network is checked against outputs of the reference's own module (fixtures h1_sit_*, made with a stand-in for
 the two ``timm`` constructors it imports); the sampler loop against ``NodeCoordsDiffusionModel.sample`` run from the
-reference's real module with its normal draws recorded (fixtures h2_sit_sample_*)."""
+reference's real module with its normal draws recorded (fixtures h2_sit_sample_*).
+
+``SiT(..., attention="differential")`` is a variant of the same network that the reference does not have: its heads are pairs of
+softmax maps, q and k are normalised per head and rotated by the nodes' coordinates (attention.py).  It is differentiable, so it
+is the one to train from scratch; its weights do not go with the other's.  ``attention="softmax"``, the default, is the
+reference's network and runs as before."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, attention as attn_ops
 
 
 class _Attention(nn.Module):          # timm.models.vision_transformer.Attention's parameters (qkv with bias, proj)
     def __init__(self, dim):
         super().__init__()
         self.qkv, self.proj = nn.Linear(dim, 3 * dim), nn.Linear(dim, dim)
+
+
+class _DiffAttention(nn.Module):
+    """H pairs of heads of d: q, k [2H, d] and v [H, 2d] from one projection; q, k normalised per head and rotated by the node's
+    coordinates (the pairs of a head dealt to the axes); differential attention; the result normalised per head.  The weight of the
+    second map is exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) + its start value, which grows with the layer's number."""
+
+    def __init__(self, dim, num_heads, layer, axes, theta):
+        super().__init__()
+        self.pairs, self.d, self.theta = num_heads // 2, dim // num_heads, theta
+        self.lambda_init = 0.8 - 0.6 * math.exp(-0.3 * layer)
+        half = self.d // 2
+        self.sections = tuple(half // axes + (1 if a < half % axes else 0) for a in range(axes))
+        self.qkv, self.proj = nn.Linear(dim, 3 * dim), nn.Linear(dim, dim)
+        self.q_norm, self.k_norm, self.out_norm = (nn.Parameter(torch.ones(n)) for n in (self.d, self.d, 2 * self.d))
+        self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2 = (nn.Parameter(0.1 * torch.randn(self.d)) for _ in range(4))
+
+    def forward(self, u, pos, mask):
+        dim = u.shape[-1]
+        q, k, v = (t.unflatten(-1, s) for t, s in zip(self.qkv(u).split(dim, -1), ((2 * self.pairs, self.d),) * 2 + ((self.pairs, 2 * self.d),)))
+        q, k = attn_ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, pos, self.sections, theta=self.theta)
+        lam = torch.exp((self.lambda_q1 * self.lambda_k1).sum()) - torch.exp((self.lambda_q2 * self.lambda_k2).sum()) + self.lambda_init
+        o = attn_ops.diff_attention(q, k, v, lam, key_mask=mask)
+        o, _ = attn_ops.qk_norm_rope(o, None, self.out_norm, None)
+        return self.proj((o * (1.0 - self.lambda_init)).flatten(2))
 
 
 class _Mlp(nn.Module):
@@ -32,9 +64,9 @@ class _Mlp(nn.Module):
 
 
 class _Block(nn.Module):
-    def __init__(self, dim, hidden):
+    def __init__(self, dim, hidden, attn=None):
         super().__init__()
-        self.attn, self.mlp = _Attention(dim), _Mlp(dim, hidden)
+        self.attn, self.mlp = attn or _Attention(dim), _Mlp(dim, hidden)
         self.adaLN_modulation = nn.Sequential(nn.Identity(), nn.Linear(dim, 6 * dim))
 
 
@@ -52,17 +84,29 @@ class _Final(nn.Module):
 
 
 class SiT(nn.Module):
-    """SiT(in_channels, hidden_size, num_transformer_blocks, num_heads, mlp_ratio) -- sit_model.py:161-187."""
+    """SiT(in_channels, hidden_size, num_transformer_blocks, num_heads, mlp_ratio) -- sit_model.py:161-187.
+
+    ``attention``: "softmax" (the reference's) or "differential" (see the module's docstring; ``num_heads`` even, heads of a
+    multiple of 8 up to 64 wide; ``rope_theta``: base of the rotation by coordinates)."""
 
     def __init__(self, in_channels=3, hidden_size=192, num_transformer_blocks=6, num_heads=6, mlp_ratio=4.0, noise_steps=1000,
-                 beta_start=1e-4, beta_end=0.02):
+                 beta_start=1e-4, beta_end=0.02, attention="softmax", rope_theta=100.0):
         super().__init__()
+        if attention not in ("softmax", "differential"):
+            raise _lib.ScggError(f"SiT: attention is 'softmax' or 'differential', got {attention!r}")
+        self.attention = attention
+        differential = attention == "differential"
+        if differential and (num_heads % 2 or hidden_size % num_heads or (hidden_size // num_heads) % 8 or hidden_size // num_heads > 64):
+            raise _lib.ScggError(f"SiT: {num_heads} heads on {hidden_size} channels: differential attention takes an even number of heads "
+                                 "of a multiple of 8 up to 64 channels")
         self.in_channels, self.hidden_size, self.num_heads = in_channels, hidden_size, num_heads
         self.mlp_hidden = int(hidden_size * mlp_ratio)
         self.noise_steps, self.beta_start, self.beta_end = noise_steps, beta_start, beta_end
         self.pos_embedder = nn.Linear(in_channels, hidden_size)
         self.t_embedder = _TEmb(hidden_size)
-        self.blocks = nn.ModuleList([_Block(hidden_size, self.mlp_hidden) for _ in range(num_transformer_blocks)])
+        self.blocks = nn.ModuleList([
+            _Block(hidden_size, self.mlp_hidden, _DiffAttention(hidden_size, num_heads, i, in_channels, rope_theta) if differential else None)
+            for i in range(num_transformer_blocks)])
         self.final_layer = _Final(hidden_size, in_channels)
         self._engine, self._key, self._versions, self._ws = None, None, None, {}
 
@@ -111,11 +155,58 @@ class SiT(nn.Module):
         off = (-ws.data_ptr()) % 256
         return C.c_void_p(ws.data_ptr() + off), ws.numel() - 256
 
-    @torch.no_grad()
     def forward(self, x, t, padding_mask):
-        """x [B,N,3], t [B] timesteps, padding_mask [B,N] bool -> predicted noise [B,N,3] (valid rows; 0 on padded ones)."""
+        """x [B,N,3], t [B] timesteps, padding_mask [B,N] bool -> predicted noise [B,N,3] (valid rows; 0 on padded ones).
+        Differentiable in the parameters and x (through its embedding; the rotation takes it as given) with differential attention,
+        forward only with the reference's."""
         if not x.is_cuda:
             raise _lib.ScggError("SiT.forward runs on the MI355X only; move the inputs to the GPU")
+        if self.attention == "differential":
+            return self._forward_differential(x, t, padding_mask)
+        return self._forward_engine(x, t, padding_mask)
+
+    def _forward_differential(self, x, t, padding_mask):
+        x, mask = x.float(), padding_mask.to(torch.bool)
+        dim = self.hidden_size
+        half = self.t_embedder.mlp[0].in_features // 2
+        arg = t.float()[:, None] * torch.exp(torch.arange(half, device=x.device) * (-math.log(10000.0) / half))
+        mlp = self.t_embedder.mlp
+        c = F.silu(mlp[2](F.silu(mlp[0](torch.cat((arg.cos(), arg.sin()), -1)))))
+        pos, h = x.detach(), self.pos_embedder(x)
+
+        def modulated(h, shift, scale):
+            return F.layer_norm(h, (dim,), eps=1e-6) * (1 + scale[:, None]) + shift[:, None]
+        for blk in self.blocks:
+            sh1, sc1, g1, sh2, sc2, g2 = blk.adaLN_modulation[1](c).chunk(6, -1)
+            h = h + g1[:, None] * blk.attn(modulated(h, sh1, sc1), pos, mask)
+            h = h + g2[:, None] * blk.mlp.fc2(F.gelu(blk.mlp.fc1(modulated(h, sh2, sc2)), approximate="tanh"))
+        sh, sc = self.final_layer.adaLN_modulation[1](c).chunk(2, -1)
+        return self.final_layer.linear(modulated(h, sh, sc)) * mask[..., None]
+
+    @torch.no_grad()
+    def _sample_differential(self, x_T, node_mask, steps, noise, seed, graph_id_base):
+        """The reference's ancestral chain (cow_diff_nodes_with_3d_checks.py:63-81), one denoiser call and one update per step; the
+        draws are those of ``scgg_sit_sample``: Philox normals keyed by (seed, global graph id, node, step), or ``noise``."""
+        beta = torch.linspace(self.beta_start, self.beta_end, self.noise_steps)
+        alpha = 1.0 - beta
+        alpha_hat = torch.cumprod(alpha, 0)
+        x, mask = x_T.detach().float().contiguous(), node_mask.to(torch.bool)
+        B, n = x.shape[:2]
+        z = torch.empty_like(x)
+        for k, i in enumerate(range(self.noise_steps - 1, 0, -1)):
+            if 0 <= steps <= k:
+                break
+            eps = self._forward_differential(x, torch.full((B,), i, device=x.device), mask)
+            al, ah, be = float(alpha[i]), float(alpha_hat[i]), float(beta[i])
+            x = (x - (1.0 - al) / math.sqrt(1.0 - ah) * eps) / math.sqrt(al)
+            if i > 1:
+                if noise is None and z.numel():
+                    _lib.check(_lib.lib().scgg_philox_normal_rows(_lib.ptr(z), B, n, seed, graph_id_base, i, _lib.stream_ptr()), "philox_normal_rows")
+                x = x + math.sqrt(be) * (z if noise is None else noise[k].float())
+        return x * mask[..., None]
+
+    @torch.no_grad()
+    def _forward_engine(self, x, t, padding_mask):
         B, n = x.shape[0], x.shape[1]
         eng = self._ensure_engine(x.device)
         ws, nb = self._workspace(B, n, x.device)
@@ -129,6 +220,8 @@ class SiT(nn.Module):
 
     @torch.no_grad()
     def sample(self, x_T, node_mask, steps=-1, noise=None, seed=0, graph_id_base=0):
+        if self.attention == "differential":
+            return self._sample_differential(x_T, node_mask, steps, noise, seed, graph_id_base)
         B, n = x_T.shape[0], x_T.shape[1]
         eng = self._ensure_engine(x_T.device)
         ws, nb = self._workspace(B, n, x_T.device)
@@ -151,9 +244,9 @@ class NodeCoordsDiffusionModel:
 
     takes_rng = True     # sample() accepts (seed, graph_id_base): NoiseModel.sample_limit_dist hands its Philox key on
 
-    def __init__(self, noise_steps=1000, beta_start=1e-4, beta_end=0.02, coordinate_size=3, device="cuda"):
+    def __init__(self, noise_steps=1000, beta_start=1e-4, beta_end=0.02, coordinate_size=3, device="cuda", attention="softmax"):
         self.model = SiT_models["SiT-T"](in_channels=coordinate_size, noise_steps=noise_steps, beta_start=beta_start,
-                                         beta_end=beta_end).to(device)
+                                         beta_end=beta_end, attention=attention).to(device)
         self.noise_steps, self.beta_start, self.beta_end, self.device = noise_steps, beta_start, beta_end, device
 
     def to_cuda_device(self, device):

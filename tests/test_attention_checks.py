@@ -135,3 +135,10 @@ def test_diff_c_entry_refuses_pointers_alignment_and_workspace():
     assert need > 0
     assert L.scgg_diff_attention_forward(C.byref(a), 4096, need - 1, None) != 0 and "workspace" in L.scgg_last_error().decode()
     assert L.scgg_diff_attention_backward(C.byref(a), None, 0, None) != 0 and "workspace" in L.scgg_last_error().decode()
+
+
+def test_sit_refuses_heads_that_do_not_pair():
+    from semantically_consistent_graph_generation_amd.node_coordinate_diffusion import SiT
+    for kw in (dict(num_heads=3), dict(num_heads=5), dict(hidden_size=768, num_heads=4), dict(hidden_size=72, num_heads=6), dict(attention="other")):
+        with pytest.raises(_lib.ScggError, match="SiT"):
+            SiT(**{"attention": "differential", **kw})

@@ -1,0 +1,81 @@
+"""SiT(attention="differential"): the model that uses the attention operators, against oracle/attention.py:sit_differential in 64 bits.
+Tolerance 1e-4 of the scale (max |a - b| / max |b|), as for the other engines of the repository: fp32 products of 192 to 768 terms and
+the operators' own bounds stay two orders below it."""
+import pytest
+import torch
+
+from oracle import attention as O
+from oracle import fixtures as fx
+from oracle import sit as S
+
+pytestmark = pytest.mark.gpu
+REL = 1e-4
+
+
+def build(name="SiT-T", seed=701, **kw):
+    from semantically_consistent_graph_generation_amd.node_coordinate_diffusion import SiT_models
+    model = SiT_models[name](in_channels=3, attention="differential", **kw)
+    sd = fx.make_state_dict({k: tuple(v.shape) for k, v in model.state_dict().items()}, seed=seed)
+    model.load_state_dict(sd)
+    return model.cuda()
+
+
+def rel(a, b):
+    return float((a.detach().double().cpu() - b.detach().double().cpu()).abs().max() / b.detach().abs().max().clamp(min=1e-30))
+
+
+def wide(model):
+    return {k: v.detach().double().requires_grad_() for k, v in model.state_dict().items()}
+
+
+@pytest.mark.parametrize("name,heads,n_nodes", [("SiT-T", 6, [40, 17, 1]), ("SiT-VT", 4, [33, 70]), ("SiT-S", 6, [9, 5, 12, 1])])
+def test_forward_and_gradients(name, heads, n_nodes):
+    model = build(name)
+    m = fx.ragged_mask(n_nodes).cuda()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(*m.shape, 3, generator=g, device="cuda", requires_grad=True)
+    t = torch.tensor([999, 500, 3, 1][: len(n_nodes)], device="cuda")
+    out = model(x, t, m)
+    sd = wide(model)
+    x64 = x.detach().double().requires_grad_()
+    want = O.sit_differential(sd, x64, t, m, len(model.blocks), heads)
+    assert rel(out, want) < REL and not out[~m].any()
+    do = torch.randn(out.shape, generator=g, device="cuda")
+    params = dict(model.named_parameters())
+    names = list(params)
+    grads = torch.autograd.grad(out, [x] + [params[k] for k in names], do)
+    wants = torch.autograd.grad(want, [x64] + [sd[k] for k in names], do.double())
+    for k, a, b in zip(["x"] + names, grads, wants):
+        assert rel(a, b) < 10 * REL, k                       # sums over all nodes of 12 sub-layers' rounding
+
+
+def test_sampler():
+    """Three steps with given draws and a whole short chain against the loop in 64 bits; Philox draws are the engine's."""
+    model = build(noise_steps=6)
+    m = fx.ragged_mask([9, 5, 12, 1]).cuda()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    xT, noise = torch.randn(*m.shape, 3, generator=g, device="cuda"), torch.randn(5, *m.shape, 3, generator=g, device="cuda")
+    sd = {k: v.detach() for k, v in wide(model).items()}
+    beta, alpha, alpha_hat = S.schedule(6)
+    for steps in (3, -1):
+        out = model.sample(xT, m, steps=steps, noise=noise)
+        x = xT.double()
+        for k, i in enumerate([5, 4, 3, 2, 1][: steps if steps > 0 else 5]):
+            eps = O.sit_differential(sd, x, torch.full((4,), i, device="cuda"), m, 6, 6)
+            x = (x - float((1 - alpha[i]) / torch.sqrt(1 - alpha_hat[i])) * eps) / float(torch.sqrt(alpha[i]))
+            x = x + (float(torch.sqrt(beta[i])) * noise[k].double() if i > 1 else 0)
+        assert rel(out, x * m[..., None]) < REL
+    a, b = model.sample(xT, m, seed=11), model.sample(xT, m, seed=11)
+    one = model.sample(xT[2:3], m[2:3], seed=11, graph_id_base=2)
+    assert torch.equal(a, b) and rel(one[0], a[2]) < 1e-5
+    assert not torch.equal(a, model.sample(xT, m, seed=12)) and not a[~m].any()
+
+
+def test_coordinate_model_and_default():
+    """NodeCoordsDiffusionModel takes the variant; the default network has the reference's parameters and nothing else."""
+    from semantically_consistent_graph_generation_amd.node_coordinate_diffusion import NodeCoordsDiffusionModel, SiT
+    cm = NodeCoordsDiffusionModel(noise_steps=4, attention="differential")
+    m = fx.ragged_mask([7, 3]).cuda()
+    out = cm.sample(torch.randn(2, 7, 3, device="cuda"), m, seed=1)
+    assert out.shape == (2, 7, 3) and torch.isfinite(out).all()
+    assert not any("norm" in k or "lambda" in k for k in SiT().state_dict())
