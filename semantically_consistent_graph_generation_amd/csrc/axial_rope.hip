@@ -10,7 +10,9 @@
 // and sines of the tile, each once for all heads of q and k: positions reach 1e6 and beyond, so the angle is a product in
 // 64 bits, reduced to an eighth of a turn there, and only then rounded to 32.  Then the heads stream through, 16 B per load: a
 // head belongs to a power of two of lanes that hold whole pairs, so the rotation needs no exchange and the norm one butterfly.
-// Statistics and products are 32-bit, each output is rounded once.  The weight gradients are summed per lane (a lane keeps
+// In the backward of a norm a workgroup belongs to q or to
+// k, so that a lane has one side's weights and sums (157 -> 142 registers; 281 -> 258 us for 4 x 16384 tokens of 20 bf16 heads of 128); elsewhere
+// it takes both, and the cosines are formed once (21 against 25 us for 27648 tokens of 16 heads of 64).  Statistics and products are 32-bit, each output is rounded once.  The weight gradients are summed per lane (a lane keeps
 // its channels), per workgroup through LDS, and over the workgroups by a second kernel in a fixed order: no atomics, equal
 // calls give equal bits.
 #include <hip/hip_runtime.h>
@@ -24,20 +26,24 @@ namespace scgg {
 namespace {
 
 constexpr int ROPE_MAX_PAIRS = 128;      // head width up to 256
-constexpr int ROPE_TILE = 16;            // tokens per workgroup tile at most
-constexpr int ROPE_TRAIN_GROUPS = 1024;  // workgroups of a backward with weights: rows of the partial sums
+constexpr int ROPE_TILE = 64;            // tokens per workgroup tile at most
+constexpr int ROPE_TRAIN_GROUPS = 2048;  // workgroups of a backward with weights, q's and k's: rows of the partial sums
 
+struct RopeSide {
+  const void* x;               // q or k as the forward takes it (backward with weights: again; without: unused)
+  const void* g;               // backward: gradient of the output
+  void* y;                     // forward: output; backward: gradient of q or k.  [B,N,heads,D] contiguous
+  const void* w;               // norm weight [D] or null
+  long long xb, xn, xh, gb, gn, gh;
+  int heads, tile;             // tokens per tile
+  unsigned blocks;             // workgroups
+};
 struct RopeArgs {
-  const void* x[2];            // q, k as the forward takes them (backward with weights: again; without: unused)
-  const void* g[2];            // backward: gradients of the outputs
-  void* y[2];                  // forward: outputs; backward: gradients of q, k.  [B,N,heads,D] contiguous
-  const void* w[2];            // norm weights [D] or null
-  long long xb[2], xn[2], xh[2], gb[2], gn[2], gh[2];
+  RopeSide side[2];            // q, k; where they have workgroups of their own, q's come first
   const void* pos;
   long long pb, pn, pa;
-  float* partial;              // [gridDim.x][2][D]
-  int heads[2];
-  int N, D, pairs, tile, pos_type, w_f32, interleaved, lanes;
+  float* partial;              // [gridDim.x][D]
+  int N, D, pairs, pos_type, w_f32, interleaved, lanes;
   int flat;                    // every batch stride is N token strides: the token's number is its place
   unsigned tokens;
   float eps;
@@ -66,16 +72,17 @@ __device__ __forceinline__ double rope_position(const RopeArgs& a, unsigned tok,
   return (double)static_cast<const int64_t*>(a.pos)[at];
 }
 
-// cos and sin of `turns` whole turns: the nearest quarter turn comes off in 64 bits, so the rounding to 32 happens to an angle of at
-// most an eighth of a turn (2^-28 of a turn), and the quarter is a swap
+// cos and sin of `turns` whole turns.  The nearest quarter turn comes off in 64 bits (adding 1.5 2^52 rounds to a whole number and leaves
+// it in the low word), so the rounding to 32 happens to an angle of at most an eighth of a turn, where the series of sin and cos need
+// five terms each: the first term left out is below x^11 / 11! = 2e-9.  The quarter is a swap and two signs.
 __device__ __forceinline__ float2 rope_cos_sin(double turns) {
-  const double q = rint(4.0 * turns);
-  const float f = (float)(turns - 0.25 * q);
-  float s, c;
-  sincospif(2.0f * f, &s, &c);
-  const int k = (int)(q - 4.0 * floor(0.25 * q));     // 0..3 (NaN and infinite positions: f and so c, s are NaN)
+  const double big = 6755399441055744.0, t = fma(4.0, turns, big), q = t - big;
+  const int k = __double2loint(t);
+  const float x = 6.283185307179586f * (float)fma(-0.25, q, turns), y = x * x;
+  const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 2.755731922e-6f, -1.984126984e-4f), 8.333333333e-3f), -1.666666667e-1f), x);
+  const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -2.755731922e-7f, 2.480158730e-5f), -1.388888889e-3f), 4.166666667e-2f), -0.5f), 1.f);
   const float cs = (k & 1) ? s : c, sn = (k & 1) ? c : s;
-  return make_float2((k == 1 || k == 2) ? -cs : cs, (k & 2) ? -sn : sn);
+  return make_float2(((k + 1) & 2) ? -cs : cs, (k & 2) ? -sn : sn);
 }
 
 template <class T>
@@ -91,7 +98,11 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   float2* cs = reinterpret_cast<float2*>(rope_lds);                       // [tile][D/2]
   const int tid = threadIdx.x, L = a.lanes, half = a.D >> 1;
   const int chunks = half / V, group = tid / L, groups = 256 / L, lane = tid - group * L;
-  const int heads = a.heads[0] + a.heads[1];
+  constexpr bool APART = NORM && BWD;                                      // q and k in workgroups of their own
+  constexpr int SIDES = APART ? 1 : 2;
+  const bool is_k = APART && blockIdx.x >= a.side[0].blocks;
+  const RopeSide& mine = is_k ? a.side[1] : a.side[0];
+  const unsigned block = blockIdx.x - (is_k ? a.side[0].blocks : 0u);
   int c0[CH], c1[CH];                                                     // element offsets of the lane's pairs: (c0 + i, c1 + i) or neighbours
   bool on[CH];
 #pragma unroll
@@ -101,52 +112,54 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     c0[c] = a.interleaved ? 2 * V * ch : V * ch;
     c1[c] = a.interleaved ? c0[c] + V : c0[c] + half;
   }
-  float w[2][CH][2 * V], dw[2][CH][2 * V];
+  float w[SIDES][CH][2 * V], dw[CH][2 * V];
   if (NORM) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < SIDES; ++s) {
+      const RopeSide& q = APART ? mine : a.side[s];
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const bool have = on[c] && a.heads[s] > 0;
-          w[s][c][i] = have ? rope_weight<T>(a.w[s], a.w_f32, c0[c] + i) : 0.f;
-          w[s][c][V + i] = have ? rope_weight<T>(a.w[s], a.w_f32, c1[c] + i) : 0.f;
-          if (BWD) dw[s][c][i] = dw[s][c][V + i] = 0.f;
+          const bool have = on[c] && q.heads > 0;
+          w[s][c][i] = have ? rope_weight<T>(q.w, a.w_f32, c0[c] + i) : 0.f;
+          w[s][c][V + i] = have ? rope_weight<T>(q.w, a.w_f32, c1[c] + i) : 0.f;
+          if (BWD) dw[c][i] = dw[c][V + i] = 0.f;
         }
+    }
   }
   const float inv_d = 1.0f / (float)a.D;
+  const int q_heads = a.side[0].heads, heads = APART ? mine.heads : q_heads + a.side[1].heads;
   const int dk = groups / heads, dh = groups - dk * heads, k_first = group / heads, h_first = group - k_first * heads;
-  const unsigned tiles = (a.tokens + a.tile - 1) / a.tile;
-  for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const unsigned tok0 = t * a.tile;
-    const int count = (int)min(a.tokens - tok0, (unsigned)a.tile);
+  const unsigned tiles = (a.tokens + mine.tile - 1) / mine.tile;
+  for (unsigned t = block; t < tiles; t += mine.blocks) {
+    const unsigned tok0 = t * mine.tile;
+    const int count = (int)min(a.tokens - tok0, (unsigned)mine.tile);
     if (a.pairs > 0) {
       __syncthreads();                                                    // the previous tile's readers are done
       for (int i = tid; i < count * half; i += 256) {
-        const int k = i / half, p = i - k * half;
+        const int k = i / half, pair = i - k * half;
         float2 v = make_float2(1.f, 0.f);
-        if (p < a.pairs) {
-          v = rope_cos_sin(rope_position(a, tok0 + k, a.axis[p]) * a.turn[p]);
+        if (pair < a.pairs) {
+          v = rope_cos_sin(rope_position(a, tok0 + k, a.axis[pair]) * a.turn[pair]);
         }
         cs[i] = v;
       }
       __syncthreads();
     }
-    int k = k_first, h = h_first;                                         // token of the tile, head among q's and k's
+    int k = k_first, h = h_first;                                         // token of the tile, head
     while (k < count) {                                                   // uniform over the L lanes of a head
-      const bool s = h >= a.heads[0];                                     // a head of k
-      const int hh = s ? h - a.heads[0] : h;
       const unsigned tok = tok0 + k;
       long long b, n;
       rope_place(a, tok, b, n);
+      const bool s = APART ? is_k : h >= q_heads;
+      const int hh = APART || !s ? h : h - q_heads;
+      const RopeSide& q = a.side[0];
+      const RopeSide& kk = a.side[1];
       const T* xp = (BWD && !NORM) ? nullptr
-                                   : static_cast<const T*>(s ? a.x[1] : a.x[0]) + b * (s ? a.xb[1] : a.xb[0]) +
-                                         n * (s ? a.xn[1] : a.xn[0]) + hh * (s ? a.xh[1] : a.xh[0]);
-      const T* gp = BWD ? static_cast<const T*>(s ? a.g[1] : a.g[0]) + b * (s ? a.gb[1] : a.gb[0]) + n * (s ? a.gn[1] : a.gn[0]) +
-                              hh * (s ? a.gh[1] : a.gh[0])
-                        : nullptr;
-      T* yp = static_cast<T*>(s ? a.y[1] : a.y[0]) + ((long long)tok * (s ? a.heads[1] : a.heads[0]) + hh) * a.D;
+                                   : static_cast<const T*>(s ? kk.x : q.x) + b * (s ? kk.xb : q.xb) + n * (s ? kk.xn : q.xn) + hh * (s ? kk.xh : q.xh);
+      const T* gp = BWD ? static_cast<const T*>(s ? kk.g : q.g) + b * (s ? kk.gb : q.gb) + n * (s ? kk.gn : q.gn) + hh * (s ? kk.gh : q.gh) : nullptr;
+      T* yp = static_cast<T*>(s ? kk.y : q.y) + ((long long)tok * (s ? kk.heads : q.heads) + hh) * a.D;
       float x[CH][2 * V], g[CH][2 * V];
       float ss = 0.f;
 #pragma unroll
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
         float* z = BWD ? g[c] : x[c];
         if (NORM && !BWD) {
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) z[i] = z[i] * r * (s ? w[1][c][i] : w[0][c][i]);
+          for (int i = 0; i < 2 * V; ++i) z[i] = z[i] * r * (!APART && s ? w[SIDES - 1][c][i] : w[0][c][i]);
         }
         if (a.interleaved) {
           // elements e = 0 .. 2V-1 of the lane are neighbours: pair i is (2i, 2i + 1)
@@ -214,12 +227,11 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 #pragma unroll
           for (int i = 0; i < 2 * V; ++i) {
             const float hx = x[c][i] * r;
-            const float du = z[i] * hx, ws = s ? w[1][c][i] : w[0][c][i];
-            dw[0][c][i] += s ? 0.f : du;
-            dw[1][c][i] += s ? du : 0.f;
-            dot = fmaf(du, ws, dot);
+            const float du = z[i] * hx;
+            dw[c][i] += du;
+            dot = fmaf(du, w[0][c][i], dot);
             x[c][i] = hx;
-            z[i] *= ws;
+            z[i] *= w[0][c][i];
           }
         }
       }
@@ -247,42 +259,41 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     }
   }
   if (NORM && BWD) {
-    // the workgroup's sums: [groups][D] of LDS per side, groups added in order
+    // the workgroup's sums: [groups][D] of LDS, groups added in order
     float* red = reinterpret_cast<float*>(rope_lds);
+    __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      __syncthreads();
+    for (int c = 0; c < CH; ++c)
+      if (on[c]) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (on[c]) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) { red[group * a.D + c0[c] + i] = dw[s][c][i]; red[group * a.D + c1[c] + i] = dw[s][c][V + i]; }
-        }
-      __syncthreads();
-      for (int d = tid; d < a.D; d += 256) {
-        float v = 0.f;
-        for (int q = 0; q < groups; ++q) v += red[q * a.D + d];
-        a.partial[((long long)blockIdx.x * 2 + s) * a.D + d] = v;
+        for (int i = 0; i < V; ++i) { red[group * a.D + c0[c] + i] = dw[c][i]; red[group * a.D + c1[c] + i] = dw[c][V + i]; }
       }
+    __syncthreads();
+    for (int d = tid; d < a.D; d += 256) {
+      float v = 0.f;
+      for (int q = 0; q < groups; ++q) v += red[q * a.D + d];
+      a.partial[(long long)blockIdx.x * a.D + d] = v;
     }
   }
 }
 
-// out[s][d] = sum of the workgroups' partials: 16 columns x 16 row lanes per workgroup, lanes added in order
+// gradient of a weight = sum of its workgroups' partials (rows [0, split) are q's, [split, rows) k's): 16 columns x 64 row lanes per
+// workgroup, lanes added in order
 template <class T>
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ partial, int rows, int D, int w_f32, void* dw0, void* dw1) {
-  __shared__ float red[16][17];
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15), rl = threadIdx.x >> 4;
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ partial, int split, int rows, int D, int w_f32, void* dw0, void* dw1) {
+  __shared__ float red[64][17];
+  const int d = blockIdx.x * 16 + (threadIdx.x & 15), rl = threadIdx.x >> 4;
+  const int from = blockIdx.y == 0 ? 0 : split, to = blockIdx.y == 0 ? split : rows;
   float v = 0.f;
-  if (c < 2 * D)
-    for (int r = rl; r < rows; r += 16) v += partial[(long long)r * 2 * D + c];
+  if (d < D) {
+#pragma unroll 4
+    for (int r = from + rl; r < to; r += 64) v += partial[(long long)r * D + d];
+  }
   red[rl][threadIdx.x & 15] = v;
   __syncthreads();
-  if (rl != 0 || c >= 2 * D) return;
-  for (int q = 1; q < 16; ++q) v += red[q][threadIdx.x & 15];
-  void* o = c < D ? dw0 : dw1;
-  if (o == nullptr) return;
-  const int d = c < D ? c : c - D;
+  void* o = blockIdx.y == 0 ? dw0 : dw1;
+  if (rl != 0 || d >= D || o == nullptr) return;
+  for (int q = 1; q < 64; ++q) v += red[q][threadIdx.x & 15];
   if (w_f32) static_cast<float*>(o)[d] = v;
   else static_cast<T*>(o)[d] = (T)v;
 }
@@ -311,8 +322,8 @@ int rope_lanes(int chunks) {
   return L;
 }
 
-// The plan of a call: elements per load, lanes per head, tokens per tile, workgroups.
-struct RopePlan { int vec, lanes, tile; long long blocks; size_t lds; };
+// The plan of a call: elements per load, lanes per head, and for q and k tokens per tile and workgroups.
+struct RopePlan { int vec, lanes, tile[2]; long long blocks[2]; size_t lds; };
 void rope_plan(const scgg_rope_args* p, bool bwd, bool norm, RopePlan* out) {
   const int size = p->dtype == SCGG_F32 ? 4 : 2, half = p->D / 2, wide = 16 / size;
   auto fits = [&](int v) {   // every row of every head starts at a multiple of the load's width
@@ -330,13 +341,31 @@ void rope_plan(const scgg_rope_args* p, bool bwd, bool norm, RopePlan* out) {
   out->vec = fits(wide) ? wide : fits(2) ? 2 : 1;
   out->lanes = rope_lanes(half / out->vec);
   const long long tokens = (long long)p->B * p->N;
-  // long inputs: 16 tokens share a tile's set-up; short ones: one token each, over as many workgroups as there are
-  long long tile = tokens / 1024;
-  out->tile = (int)(tile < 1 ? 1 : tile > ROPE_TILE ? ROPE_TILE : tile);
-  const long long tiles = (tokens + out->tile - 1) / out->tile;
-  const long long cap = bwd && norm ? ROPE_TRAIN_GROUPS : tiles;
-  out->blocks = tiles < cap ? tiles : cap;
-  out->lds = p->n_sections > 0 ? (size_t)out->tile * half * sizeof(float2) : 0;
+  out->lds = 0;
+  const long long all = (long long)p->heads[0] + p->heads[1];
+  const bool apart = bwd && norm;
+  for (int s = 0; s < 2; ++s) {
+    // long inputs: a tile has about twelve heads for each group of lanes, and its cosines fill 16 KiB at most; shorter ones: smaller
+    // tiles, so that there are some 1500 workgroups (q's and k's by their heads), down to one token each
+    const long long own = apart ? p->heads[s] : s == 0 ? all : 0;
+    out->tile[s] = 1;
+    out->blocks[s] = 0;
+    if (own == 0 || tokens == 0) continue;
+    const long long many = tokens * all / own / 1536, turn = 12 * 256 / out->lanes / own + 1, room = 2048 / half;
+    long long tile = many < turn ? many : turn;
+    if (tile > room) tile = room;
+    if (tile > ROPE_TILE) tile = ROPE_TILE;
+    if (tile < 1) tile = 1;
+    const long long groups = 256 / out->lanes;
+    auto idle = [&](long long t) { return (double)((t * own + groups - 1) / groups * groups) / (double)(t * own); };
+    for (long long t = tile, least = tile / 2 + 1; t >= least; --t)         // of the sizes down to half: the one whose last round is fullest
+      if (idle(t) < idle(tile) - 1e-9) tile = t;
+    const long long tiles = (tokens + tile - 1) / tile, cap = apart ? ROPE_TRAIN_GROUPS * own / all : tiles;
+    out->tile[s] = (int)tile;
+    out->blocks[s] = tiles < cap ? tiles : cap < 1 ? 1 : cap;
+    const size_t lds = p->n_sections > 0 ? (size_t)tile * half * sizeof(float2) : 0;
+    if (lds > out->lds) out->lds = lds;
+  }
   if (bwd && norm) {
     const size_t red = (size_t)(256 / out->lanes) * p->D * sizeof(float);
     if (red > out->lds) out->lds = red;
@@ -381,15 +410,18 @@ int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspac
   }
   RopePlan plan;
   rope_plan(p, bwd, norm, &plan);
-  if ((long long)p->heads[0] + p->heads[1] == 0) plan.blocks = 0;
   RopeArgs a = {};
+  const long long blocks = plan.blocks[0] + plan.blocks[1];
+  if (blocks > 0x7fffffffLL) return fail("%s: too many tokens for one launch", what);
   for (int s = 0; s < 2; ++s) {
-    a.x[s] = p->x[s]; a.g[s] = p->g[s]; a.y[s] = p->y[s]; a.w[s] = p->weight[s]; a.heads[s] = p->heads[s];
-    a.xb[s] = p->x_stride_b[s]; a.xn[s] = p->x_stride_n[s]; a.xh[s] = p->x_stride_h[s];
-    a.gb[s] = p->g_stride_b[s]; a.gn[s] = p->g_stride_n[s]; a.gh[s] = p->g_stride_h[s];
+    RopeSide& q = a.side[s];
+    q.x = p->x[s]; q.g = p->g[s]; q.y = p->y[s]; q.w = p->weight[s]; q.heads = p->heads[s];
+    q.xb = p->x_stride_b[s]; q.xn = p->x_stride_n[s]; q.xh = p->x_stride_h[s];
+    q.gb = p->g_stride_b[s]; q.gn = p->g_stride_n[s]; q.gh = p->g_stride_h[s];
+    q.tile = plan.tile[s]; q.blocks = (unsigned)plan.blocks[s];
   }
   a.pos = p->positions; a.pb = p->pos_stride_b; a.pn = p->pos_stride_n; a.pa = p->pos_stride_a; a.pos_type = p->pos_type;
-  a.N = p->N > 0 ? p->N : 1; a.D = p->D; a.tile = plan.tile; a.w_f32 = p->weight_f32; a.interleaved = p->interleaved != 0;
+  a.N = p->N > 0 ? p->N : 1; a.D = p->D; a.w_f32 = p->weight_f32; a.interleaved = p->interleaved != 0;
   a.lanes = plan.lanes; a.tokens = (unsigned)(p->B * p->N); a.eps = p->eps;
   a.flat = 1;
   for (int s = 0; s < 2; ++s) {
@@ -405,23 +437,23 @@ int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspac
     }
   if (a.pairs == 0 && !(bwd && norm)) plan.lds = 0;
   if (bwd && norm) {
-    const size_t need = (size_t)plan.blocks * 2 * p->D * sizeof(float);
+    const size_t need = (size_t)blocks * p->D * sizeof(float);
     if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
     a.partial = static_cast<float*>(workspace);
   }
-  if (plan.blocks > 0) {
-    if (p->dtype == SCGG_F32) rope_launch<float>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
-    else if (p->dtype == SCGG_BF16) rope_launch<__bf16>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
-    else rope_launch<_Float16>(a, plan.vec, norm, bwd, (unsigned)plan.blocks, plan.lds, st);
+  if (blocks > 0) {
+    if (p->dtype == SCGG_F32) rope_launch<float>(a, plan.vec, norm, bwd, (unsigned)blocks, plan.lds, st);
+    else if (p->dtype == SCGG_BF16) rope_launch<__bf16>(a, plan.vec, norm, bwd, (unsigned)blocks, plan.lds, st);
+    else rope_launch<_Float16>(a, plan.vec, norm, bwd, (unsigned)blocks, plan.lds, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
   }
   if (bwd && norm && (p->dweight[0] || p->dweight[1])) {
-    const dim3 grid((unsigned)((2 * p->D + 15) / 16));
-    const int rows = (int)plan.blocks;   // none: the sums are zero
-    if (p->dtype == SCGG_F32) hipLaunchKernelGGL(rope_dw_kernel<float>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
-    else if (p->dtype == SCGG_BF16) hipLaunchKernelGGL(rope_dw_kernel<__bf16>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
-    else hipLaunchKernelGGL(rope_dw_kernel<_Float16>, grid, dim3(256), 0, st, a.partial, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    const dim3 grid((unsigned)((p->D + 15) / 16), 2);
+    const int split = (int)plan.blocks[0], rows = (int)blocks;   // none: the sums are zero
+    if (p->dtype == SCGG_F32) hipLaunchKernelGGL(rope_dw_kernel<float>, grid, dim3(1024), 0, st, a.partial, split, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    else if (p->dtype == SCGG_BF16) hipLaunchKernelGGL(rope_dw_kernel<__bf16>, grid, dim3(1024), 0, st, a.partial, split, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
+    else hipLaunchKernelGGL(rope_dw_kernel<_Float16>, grid, dim3(1024), 0, st, a.partial, split, rows, p->D, p->weight_f32, p->dweight[0], p->dweight[1]);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
   }
@@ -435,7 +467,7 @@ using namespace scgg;
 
 extern "C" size_t scgg_rope_workspace_bytes(const scgg_rope_args* p) {
   if (rope_check(p, "rope_workspace_bytes")) return 0;
-  return (size_t)ROPE_TRAIN_GROUPS * 2 * p->D * sizeof(float);
+  return (size_t)(ROPE_TRAIN_GROUPS + 2) * p->D * sizeof(float);
 }
 
 extern "C" int scgg_rope_forward(const scgg_rope_args* p, void* stream) {
