@@ -46,13 +46,14 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
 
   Frag<P> qf[2][DP / 16], gf[DVP / 16];
-  Prob<T> prob[2];
+  float mc[2], il[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     load_rows<T, DP>(qf[i], static_cast<const T*>(a.q) + b * a.qb + (long long)q * a.qn + (2ll * h + i) * a.qh, q_on, a.d, g);
     float2 st = make_float2(INFINITY, 0.f);
     if (q_on) st = a.stats[((long long)bh * 2 + i) * a.N + q];
-    prob[i] = Prob<T>(st.x, st.y, 1.f);
+    mc[i] = st.x;
+    il[i] = st.y;
   }
   load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on, a.dv_w, g);
 
@@ -125,8 +126,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
           if (part) hide(s, see, hh, g);
           float sum = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum = fmaf(prob[i](s[r], a.c), dp[r], sum);
-          delta[i] += sum;
+          for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
+          delta[i] = fmaf(sum, il[i], delta[i]);                  // dlambda is held to 32 bits: 1 / sum as a factor, not in the exponent
         }
         if (__is_same(T, _Float16)) {
 #pragma unroll
@@ -159,6 +160,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   }
   float up = 1.f;                                   // |dS| <= 2 max(1, |lambda|) max |dP|
   if (__is_same(T, _Float16)) up = pow2_below(16384.f, 2.f * fmaxf(1.f, fabsf(lam)) * top);
+  const Prob<T> prob[2] = {Prob<T>(mc[0], il[0], 1.f), Prob<T>(mc[1], il[1], 1.f)};
   const float w[2] = {up, -up * lam}, wd[2] = {-w[0] * delta[0], -w[1] * delta[1]};
 
   f32x16 o[2][ND];
