@@ -72,12 +72,13 @@ Args make(const scgg_diff_attention_args* p) {
   return a;
 }
 
-// Keys split over workgroups (0: not): when the rows of a key head's group fill no more than one block of 32 and there are keys to split
+// Keys split over workgroups (0: not): where the queries give the other kernel less than one workgroup (of 64) to every second CU, and
+// there are keys to split.  Such a kernel is one long chain of tiles on a few CUs.
 void plan_split(Args& a) {
-  const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, heads = (long long)a.B * a.Hkv;
+  const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32);
   a.splits = 0;
-  if (rows > 32 || tiles < 2 * SPLIT_MIN_TILES) return;
-  long long s = SPLIT_GROUPS / (heads > 0 ? heads : 1);
+  if ((rows > 32 && (long long)a.B * a.H * ((a.N + 63) / 64) >= 128) || tiles < 2 * SPLIT_MIN_TILES || blocks == 0) return;
+  long long s = SPLIT_GROUPS / blocks;
   if (s > tiles / SPLIT_MIN_TILES) s = tiles / SPLIT_MIN_TILES;
   if (s < 1) s = 1;
   a.split_tiles = (int)((tiles + s - 1) / s);

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
 }
 
 // A few rows against many keys: one pass over k and v, the keys split over workgroups.  The rows of a key head's group (queries x
-// heads that share it) are the columns of a 32-wide block.  A wave takes one map and one half of a tile's keys and keeps its own
+// heads that share it) are the columns of 32-wide blocks.  A wave takes one map and one half of a tile's keys and keeps its own
 // maximum, sum and P v, which split_join merges.  P is at most 1 here and not yet A, so it is taken in two terms (h + l): the
 // pass waits for memory, the products are free.
 template <class T, int DP, int DVP>
@@ -254,11 +254,11 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   char* vt = lds + KTile::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
   const int hh = wave & 1, map = wave >> 1;
-  const int group = a.H / a.Hkv, rows = a.N * group;             // at most 32
-  const int bk = blockIdx.x / a.splits, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-  const int split = (int)((blockIdx.x + bk) % a.splits);        // turned by the head: the dies (ids modulo 8) share the ends of short sequences
-  const int n = l31 / group, h = hk * group + (l31 - n * group);
-  const bool on = l31 < rows;
+  const int group = a.H / a.Hkv, rows = a.N * group, blocks = (rows + 31) / 32;
+  const int at = blockIdx.x / a.splits, bk = at / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv, row = (at - bk * blocks) * 32 + l31;
+  const int split = (int)((blockIdx.x + at) % a.splits);        // turned by the head: the dies (ids modulo 8) share the ends of short sequences
+  const int n = row / group, h = hk * group + (row - n * group);
+  const bool on = row < rows;
   const long long off = (long long)a.M - a.N;
   const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
   const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   l += __shfl_xor(l, 32);
   if (!on) return;
   const int slots = 2 * a.splits, ld = 2 * a.dv_w + 4;
-  float* out = a.part + (((long long)bk * rows + l31) * slots + 2 * split + hh) * ld;
+  float* out = a.part + (((long long)bk * rows + row) * slots + 2 * split + hh) * ld;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -417,7 +417,7 @@ int launch_split(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&split_kernel<T, DP, DVP>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.Hkv * a.splits;
+  const long long blocks = (long long)a.B * a.Hkv * (((long long)a.N * (a.H / a.Hkv) + 31) / 32) * a.splits;
   if (blocks > 0x7fffffffLL || (long long)a.B * a.N * a.H > 0x7fffffffLL) return -3;
   hipLaunchKernelGGL((split_kernel<T, DP, DVP>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(THREADS), 0, st, a);
