@@ -42,11 +42,12 @@ struct Args {
   void *out, *dq, *dk, *dv;
   float2* stats;                  // [B,H,2,N]: scale log2(e) max, 1 / sum
   float* delta;                   // [B,H,2,N]: sum_j P_i dP
-  float* part;                    // partial results of the splits (split_kernel, dkv_kernel)
+  float* part;                    // partial results of the splits (split_kernel, dq_kernel, dkv_kernel)
   long long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh, mb;
   float scale, c;                 // c = scale log2(e)
   int B, N, M, H, Hkv, d, dv_w, causal;
   int splits, split_tiles;        // forward: workgroups along the keys and the tiles each of them takes; dkv_kernel: along the queries
+  int dq_splits;                  // dq_kernel: workgroups along the keys
 };
 
 // ------------------------------------------------------------------------------------------------ element types

@@ -97,10 +97,30 @@ void plan_dkv(Args& a) {
   if (s > tiles / 4) s = tiles / 4;
   a.splits = s < 1 ? 1 : (int)s;
 }
+// Keys split over workgroups in the dQ kernel: as in the forward, where the queries (64 to a workgroup) fill less than half of the GPU.  The
+// splits' dQ and the sweeps' second launch cost about as much as eight tiles.
+void plan_dq(Args& a) {
+  const long long blocks = (long long)a.B * a.H * ((a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
+  long long s = blocks > 0 && blocks < 128 ? 512 / blocks : 1;
+  if (s > 16) s = 16;
+  if (s > tiles / 8) s = tiles / 8;
+  a.dq_splits = s < 1 ? 1 : (int)s;
+}
+size_t dq_part_bytes(const Args& a) {
+  return a.dq_splits <= 1 ? 0 : (size_t)a.dq_splits * a.B * a.H * a.N * 2 * a.d * sizeof(float);
+}
 size_t dkv_part_bytes(const Args& a) {
   return a.splits <= 1 ? 0 : (size_t)a.splits * a.B * a.M * a.Hkv * (2 * a.d + a.dv_w) * sizeof(float);
 }
 size_t delta_bytes(const Args& a) { return ((size_t)a.B * a.H * 3 * a.N * sizeof(float) + 255) / 256 * 256; }
+
+// the deltas, and the splits' parts of one kernel after the other
+size_t backward_bytes(Args& a) {
+  plan_dq(a);
+  plan_dkv(a);
+  const size_t q = dq_part_bytes(a), kv = dkv_part_bytes(a);
+  return delta_bytes(a) + (q > kv ? q : kv);
+}
 
 int done(int rc, const char* what) {
   if (rc == -3) return fail("%s: too many tokens for one launch", what);
@@ -126,8 +146,7 @@ extern "C" size_t scgg_diff_attention_forward_workspace_bytes(const scgg_diff_at
 extern "C" size_t scgg_diff_attention_backward_workspace_bytes(const scgg_diff_attention_args* p) {
   if (check(p, "diff_attention_backward_workspace_bytes")) return 0;
   Args a = make(p);
-  plan_dkv(a);
-  return delta_bytes(a) + dkv_part_bytes(a);
+  return backward_bytes(a);
 }
 
 extern "C" int scgg_diff_attention_forward(const scgg_diff_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -156,8 +175,7 @@ extern "C" int scgg_diff_attention_backward(const scgg_diff_attention_args* p, v
     return fail("%s: base and strides of dout have to be multiples of 16 bytes", what);
   if (queries && !near(p, p->dout_stride_n, 0, p->dv)) return fail("%s: rows of dout have to lie less than 2 GiB / 64 apart", what);
   Args a = make(p);
-  plan_dkv(a);
-  const size_t need = delta_bytes(a) + dkv_part_bytes(a);
+  const size_t need = backward_bytes(a);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
   a.delta = static_cast<float*>(workspace);
   a.part = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)) : nullptr;

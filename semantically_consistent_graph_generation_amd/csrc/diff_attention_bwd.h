@@ -23,8 +23,10 @@ struct DqShape {
   static constexpr int MIN_BLOCKS = P == 3 ? 1 : 2;
 };
 
-// delta [B,H,3,N]: delta_1, delta_2, and the largest |dP| of the query
-template <class T, int DP, int DVP, int KW>
+// delta [B,H,3,N]: delta_1, delta_2, and the largest |dP| of the query.
+// PHASE 0: both sweeps.  With few queries the keys are split over `dq_splits` workgroups, and the sweeps are launches of their own: 1 writes
+// the splits' deltas to `part` (delta_join adds them), 2 the splits' dQ in 32 bits (dq_join).
+template <class T, int DP, int DVP, int KW, int PHASE>
 __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq_kernel(Args a) {
   typedef DqShape<T, DP, DVP> S;
   typedef typename S::KTile KTile;
@@ -35,8 +37,9 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   char* vt = lds + KTile::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l31 = lane & 31;
   const int qw = wave / KW, kw = wave - qw * KW;
-  const int q_tiles = (a.N + BQ - 1) / BQ;
-  const unsigned id = die_major(blockIdx.x, gridDim.x);
+  const int q_tiles = (a.N + BQ - 1) / BQ, splits = PHASE == 0 ? 1 : a.dq_splits;
+  const unsigned whole = die_major(blockIdx.x, gridDim.x), id = whole / splits;
+  const int split = PHASE == 0 ? 0 : (int)(whole - id * splits);
   const int bh = id / q_tiles, qt = a.causal ? q_tiles - 1 - (int)(id - bh * q_tiles) : (int)(id - bh * q_tiles);
   const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
   const int q = qt * BQ + 32 * qw + l31;
@@ -68,6 +71,12 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
     if (e < keys.end) keys.end = e;
   }
   const long long wave_last = (long long)qt * BQ + 32 * qw + 31 + off;
+  int first = 0;
+  if constexpr (PHASE != 0) {
+    const int tiles = keys.end;
+    first = (int)((long long)tiles * split / splits);
+    keys.end = (int)((long long)tiles * (split + 1) / splits);
+  }
 
   Stage<T, 2 * DP, 2> ks;
   Stage<T, DVP, 1> vs;
@@ -87,8 +96,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   };
   auto seen = [&](int t, u64 bits) { return a.causal ? bits & upto(q + off - (long long)t * TILE) : bits; };
   auto begin = [&](int& t, u64& bits) {
-    keys.start(0, wave, lane);
-    t = keys.next(0, bits, wave, lane);
+    keys.start(first, wave, lane);
+    t = keys.next(first, bits, wave, lane);
     if (t < keys.end) {
       ks.load(kp + (long long)t * TILE * a.kn, bits, tid);
       vs.load(vp + (long long)t * TILE * a.vn, bits, tid);
@@ -110,54 +119,62 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   float delta[2] = {0.f, 0.f}, top = 0.f;
   u64 bits, bits_next;
   int t;
-  begin(t, bits);
-  while (t < keys.end) {
-    const int tn = advance(t, bits_next);
-    if (!a.causal || (long long)t * TILE <= wave_last) {
-      const u64 see = seen(t, bits);
-      const bool part = __any(see != ~0ull);
+  if constexpr (PHASE != 2) {
+    begin(t, bits);
+    while (t < keys.end) {
+      const int tn = advance(t, bits_next);
+      if (!a.causal || (long long)t * TILE <= wave_last) {
+        const u64 see = seen(t, bits);
+        const bool part = __any(see != ~0ull);
 #pragma unroll
-      for (int half = 0; half < 2 / KW; ++half) {
-        const int hh = KW == 1 ? half : kw;
-        const f32x16 dp = dprob(hh);
+        for (int half = 0; half < 2 / KW; ++half) {
+          const int hh = KW == 1 ? half : kw;
+          const f32x16 dp = dprob(hh);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f32x16 s = score(i, hh);
-          if (part) hide(s, see, hh, g);
-          float sum = 0.f;
+          for (int i = 0; i < 2; ++i) {
+            f32x16 s = score(i, hh);
+            if (part) hide(s, see, hh, g);
+            float sum = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
-          delta[i] = fmaf(sum, il[i], delta[i]);                  // dlambda is held to 32 bits: 1 / sum as a factor, not in the exponent
-        }
-        if (__is_same(T, _Float16)) {
+            for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
+            delta[i] = fmaf(sum, il[i], delta[i]);                  // dlambda is held to 32 bits: 1 / sum as a factor, not in the exponent
+          }
+          if (__is_same(T, _Float16)) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+          }
         }
       }
+      t = tn;
+      bits = bits_next;
     }
-    t = tn;
-    bits = bits_next;
-  }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) delta[i] += __shfl_xor(delta[i], 32);
-  top = fmaxf(top, __shfl_xor(top, 32));
-  if constexpr (KW == 2) {
-    float* box = reinterpret_cast<float*>(lds);
-    __syncthreads();
-    if (g == 0) { box[(wave * 3) * 32 + l31] = delta[0]; box[(wave * 3 + 1) * 32 + l31] = delta[1]; box[(wave * 3 + 2) * 32 + l31] = top; }
-    __syncthreads();
-    const int w0 = wave & ~1;
-    delta[0] = box[(w0 * 3) * 32 + l31] + box[(w0 * 3 + 3) * 32 + l31];
-    delta[1] = box[(w0 * 3 + 1) * 32 + l31] + box[(w0 * 3 + 4) * 32 + l31];
-    top = fmaxf(box[(w0 * 3 + 2) * 32 + l31], box[(w0 * 3 + 5) * 32 + l31]);
+    for (int i = 0; i < 2; ++i) delta[i] += __shfl_xor(delta[i], 32);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if constexpr (KW == 2) {
+      float* box = reinterpret_cast<float*>(lds);
+      __syncthreads();
+      if (g == 0) { box[(wave * 3) * 32 + l31] = delta[0]; box[(wave * 3 + 1) * 32 + l31] = delta[1]; box[(wave * 3 + 2) * 32 + l31] = top; }
+      __syncthreads();
+      const int w0 = wave & ~1;
+      delta[0] = box[(w0 * 3) * 32 + l31] + box[(w0 * 3 + 3) * 32 + l31];
+      delta[1] = box[(w0 * 3 + 1) * 32 + l31] + box[(w0 * 3 + 4) * 32 + l31];
+      top = fmaxf(box[(w0 * 3 + 2) * 32 + l31], box[(w0 * 3 + 5) * 32 + l31]);
+    }
+    if (q_on && kw == 0 && g == 0) {
+      float* dst = (PHASE == 1 ? a.part + (long long)split * a.B * a.H * 3 * a.N : a.delta) + (long long)bh * 3 * a.N + q;
+      dst[0] = delta[0];
+      dst[a.N] = delta[1];
+      dst[2ll * a.N] = top;
+    }
+    if constexpr (PHASE == 1) return;
+  } else if (q_on) {
+    const float* src = a.delta + (long long)bh * 3 * a.N + q;
+    delta[0] = src[0];
+    delta[1] = src[a.N];
+    top = src[2ll * a.N];
   }
   const float lam = a.lambda[h];
-  if (q_on && kw == 0 && g == 0) {
-    float* dst = a.delta + (long long)bh * 3 * a.N + q;
-    dst[0] = delta[0];
-    dst[a.N] = delta[1];
-    dst[2ll * a.N] = top;
-  }
   float up = 1.f;                                   // |dS| <= 2 max(1, |lambda|) max |dP|
   if (__is_same(T, _Float16)) up = pow2_below(16384.f, 2.f * fmaxf(1.f, fabsf(lam)) * top);
   const Prob<T> prob[2] = {Prob<T>(mc[0], il[0], 1.f), Prob<T>(mc[1], il[1], 1.f)};
@@ -219,15 +236,47 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   const float f = a.scale / up;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    T* dst = static_cast<T*>(a.dq) + (((long long)b * a.N + q) * 2 * a.H + 2 * h + i) * a.d;
+    const long long row = ((long long)b * a.N + q) * 2 * a.H + 2 * h + i;
+    T* dst = static_cast<T*>(a.dq) + row * a.d;
+    float* part = PHASE == 2 ? a.part + ((long long)split * a.B * a.N * 2 * a.H + row) * a.d : nullptr;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int col = 32 * j + 2 * r + 4 * g;
-        if (col < a.d) store4<T>(dst + col, o[i][j][r] * f, o[i][j][r + 1] * f, o[i][j][r + 2] * f, o[i][j][r + 3] * f);
+        if (col >= a.d) continue;
+        const f32x4 v = {o[i][j][r] * f, o[i][j][r + 1] * f, o[i][j][r + 2] * f, o[i][j][r + 3] * f};
+        if constexpr (PHASE == 2) *reinterpret_cast<f32x4*>(part + col) = v;
+        else store4<T>(dst + col, v[0], v[1], v[2], v[3]);
       }
   }
+}
+
+// the splits' deltas, in order
+__global__ __launch_bounds__(256) inline void delta_join(Args a, long long rows) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows) return;
+  const long long bh = i / a.N, at = bh * 3 * a.N + (i - bh * a.N), step = rows * 3;
+  float d1 = 0.f, d2 = 0.f, top = 0.f;
+  for (int s = 0; s < a.dq_splits; ++s) {
+    const float* p = a.part + s * step + at;
+    d1 += p[0];
+    d2 += p[a.N];
+    top = fmaxf(top, p[2ll * a.N]);
+  }
+  a.delta[at] = d1;
+  a.delta[at + a.N] = d2;
+  a.delta[at + 2ll * a.N] = top;
+}
+
+// the splits' dQ of four neighbouring columns, in order
+template <class T>
+__global__ __launch_bounds__(256) void dq_join(Args a, long long quads) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.dq_splits; ++s) v += *reinterpret_cast<const f32x4*>(a.part + (s * quads + i) * 4);
+  store4<T>(static_cast<T*>(a.dq) + i * 4, v[0], v[1], v[2], v[3]);
 }
 
 template <class T, int DP, int DVP>
@@ -497,14 +546,25 @@ __global__ __launch_bounds__(256) void dkv_join(Args a, long long quads) {
   store4<T>(dst, v[0], v[1], v[2], v[3]);
 }
 
-template <class T, int DP, int DVP, int KW>
+template <class T, int DP, int DVP, int KW, int PHASE>
 int launch_dq(const Args& a, hipStream_t st) {
   typedef DqShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW, PHASE>), S::LDS)) return -2;
+  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW)) * (PHASE == 0 ? 1 : a.dq_splits);
   if (blocks > 0x7fffffffLL) return -3;
-  if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW, PHASE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  return 0;
+}
+
+template <class T, int DP, int DVP>
+int launch_dq_split(const Args& a, hipStream_t st) {
+  const long long rows = (long long)a.B * a.H * a.N, quads = rows * 2 * a.d / 4;
+  if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
+  if (const int rc = launch_dq<T, DP, DVP, 2, 1>(a, st)) return rc;
+  hipLaunchKernelGGL(delta_join, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);
+  if (const int rc = launch_dq<T, DP, DVP, 2, 2>(a, st)) return rc;
+  hipLaunchKernelGGL((dq_join<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, quads);
   return 0;
 }
 
@@ -522,7 +582,8 @@ int launch_dkv(const Args& a, hipStream_t st) {
 template <class T, int DP, int DVP>
 int launch_bwd(const Args& a, hipStream_t st) {
   const bool few_q = (long long)a.B * a.H * ((a.N + 127) / 128) < 512;
-  if (const int rc = few_q ? launch_dq<T, DP, DVP, 2>(a, st) : launch_dq<T, DP, DVP, 1>(a, st)) return rc;
+  if (const int rc = a.dq_splits > 1 ? launch_dq_split<T, DP, DVP>(a, st) : few_q ? launch_dq<T, DP, DVP, 2, 0>(a, st) : launch_dq<T, DP, DVP, 1, 0>(a, st))
+    return rc;
   if constexpr (DkvShape<T, DP, DVP>::APART) {
     if (const int rc = launch_dkv<T, DP, DVP, 1>(a, st)) return rc;
     if (const int rc = launch_dkv<T, DP, DVP, 2>(a, st)) return rc;

@@ -128,7 +128,8 @@ CASES = [  # B, N, M, H, Hkv, d, dv, mask, causal
     (2, 257, 130, 2, 2, 32, 32, "ragged", True), (2, 33, 1, 2, 1, 40, 24, "none", False), (1, 1, 640, 4, 2, 64, 128, "random", False),
     (3, 2, 1025, 6, 3, 32, 64, "ragged", True), (2, 5, 513, 4, 1, 24, 80, "none", False), (1, 9, 9000, 2, 2, 16, 16, "rare", False),
     (1, 90, 8300, 1, 1, 64, 128, "rare", False), (2, 300, 300, 8, 2, 64, 128, "ragged", True), (1, 31, 600, 2, 2, 48, 96, "rare", True),
-    (70, 7, 33, 1, 1, 32, 64, "ragged", False), (1, 1000, 140, 2, 2, 56, 104, "none", True),
+    (70, 7, 33, 1, 1, 32, 64, "ragged", False), (1, 1000, 140, 2, 2, 56, 104, "none", True), (2, 100, 2100, 2, 1, 64, 128, "ragged", True),
+    (1, 45, 1200, 3, 3, 32, 64, "random", True), (1, 1500, 1100, 2, 1, 48, 96, "none", True),
 ]
 
 
