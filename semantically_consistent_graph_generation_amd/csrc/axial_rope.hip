@@ -439,6 +439,7 @@ int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspac
   if (bwd && norm) {
     const size_t need = (size_t)blocks * p->D * sizeof(float);
     if (need > 0 && (!workspace || workspace_bytes < need)) return fail("%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail("%s: workspace has to be aligned to 16 bytes", what);
     a.partial = static_cast<float*>(workspace);
   }
   if (blocks > 0) {

@@ -253,7 +253,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
 }
 
 // the splits' deltas, in order
-__global__ __launch_bounds__(256) inline void delta_join(Args a, long long rows) {
+static __global__ __launch_bounds__(256) void delta_join(Args a, long long rows) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows) return;
   const long long bh = i / a.N, at = bh * 3 * a.N + (i - bh * a.N), step = rows * 3;

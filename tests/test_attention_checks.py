@@ -79,6 +79,7 @@ def test_rope_c_entry_refuses_missing_pointers():
     a.weight[1] = 4096
     a.g[1] = 4096
     assert L.scgg_rope_backward(C.byref(a), None, 0, None) != 0 and "workspace" in L.scgg_last_error().decode()
+    assert L.scgg_rope_backward(C.byref(a), 4100, 1 << 30, None) != 0 and "aligned" in L.scgg_last_error().decode()
     a.eps = -1.0
     assert L.scgg_rope_forward(C.byref(a), None) != 0 and "eps" in L.scgg_last_error().decode()
 
@@ -134,6 +135,11 @@ def test_diff_c_entry_refuses_pointers_alignment_and_workspace():
     need = L.scgg_diff_attention_forward_workspace_bytes(C.byref(a))
     assert need > 0
     assert L.scgg_diff_attention_forward(C.byref(a), 4096, need - 1, None) != 0 and "workspace" in L.scgg_last_error().decode()
+    assert L.scgg_diff_attention_forward(C.byref(a), 4096 + 128, need, None) != 0 and "aligned" in L.scgg_last_error().decode()
+    far = diff_args(k_stride_n=2 ** 24)
+    assert L.scgg_diff_attention_forward(C.byref(far), None, 0, None) != 0 and "2 GiB" in L.scgg_last_error().decode()
+    far = diff_args(dout_stride_n=2 ** 24)
+    assert L.scgg_diff_attention_backward(C.byref(far), 4096, 1 << 30, None) != 0 and "2 GiB" in L.scgg_last_error().decode()
     assert L.scgg_diff_attention_backward(C.byref(a), None, 0, None) != 0 and "workspace" in L.scgg_last_error().decode()
 
 
