@@ -59,6 +59,14 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
     il[i] = st.y;
   }
   load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on, a.dv_w, g);
+  // Odd queries take - dO: the matrix instructions round dP with a bias of one sign (fp16: 1e-2 of a step), and dlambda, the sum of P dP over all
+  // queries, would add it up (2e-5 of 30 over 1554 queries); so it has the other sign in every second one.
+  const float side = (l31 & 1) ? -1.f : 1.f;
+  const unsigned flip = (l31 & 1) ? 0x80008000u : 0u;
+#pragma unroll
+  for (int c = 0; c < DVP / 16; ++c)
+#pragma unroll
+    for (int i = 0; i < P; ++i) gf[c].p[i] ^= flip;
 
   KeyBits keys;
   keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
@@ -137,7 +145,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
             float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mc[i])), dp[r], sum);
-            delta[i] = fmaf(sum, il[i], delta[i]);                  // dlambda is held to 32 bits: 1 / sum as a factor, not in the exponent
+            delta[i] = fmaf(sum, side * il[i], delta[i]);                  // dlambda is held to 32 bits: 1 / sum as a factor, not in the exponent
           }
           if (__is_same(T, _Float16)) {
 #pragma unroll
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
   float up = 1.f;                                   // |dS| <= 2 max(1, |lambda|) max |dP|
   if (__is_same(T, _Float16)) up = pow2_below(16384.f, 2.f * fmaxf(1.f, fabsf(lam)) * top);
   const Prob<T> prob[2] = {Prob<T>(mc[0], il[0], 1.f), Prob<T>(mc[1], il[1], 1.f)};
-  const float w[2] = {up, -up * lam}, wd[2] = {-w[0] * delta[0], -w[1] * delta[1]};
+  const float wd[2] = {-up * delta[0], up * lam * delta[1]}, w[2] = {side * up, -side * up * lam};
 
   f32x16 o[2][ND];
 #pragma unroll
