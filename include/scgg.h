@@ -572,7 +572,7 @@ typedef struct scgg_diff_attention_args {
   const uint8_t* key_mask;             /* [B,M], dense along M; NULL: every key is seen */
   void* out;                           /* [B,N,H,dv] contiguous */
   float* stats;                        /* [B,H,2,N,2]: of each map and query the largest score (in units of the base-2
-                                          exponent) and 1 / sum; written by the forward (NULL: not wanted), read by the backward */
+                                          exponent, or one near it) and 1 / sum; written by the forward (NULL: not wanted), read by the backward */
   const void* dout;                    /* backward: [B,N,H,dv] */
   void* dq;                            /* contiguous, as are the other gradients */
   void* dk;

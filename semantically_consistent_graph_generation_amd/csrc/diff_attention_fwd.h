@@ -121,15 +121,41 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
     if (!a.causal || (long long)t * TILE <= wave_last) {
       const u64 see = seen(t, bits);
       const bool part = __any(see != ~0ull);
+      f32x16 s[2 / KW][2];
 #pragma unroll
-      for (int half = 0; half < 2 / KW; ++half) {
-        const int hh = KW == 1 ? half : kw;
+      for (int half = 0; half < 2 / KW; ++half)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          f32x16 s = score(i, hh);
-          if (part) hide(s, see, hh, g);
-          add_stats(s, a.c, m[i], l[i]);
+          s[half][i] = score(i, KW == 1 ? half : kw);
+          if (part) hide(s[half][i], see, KW == 1 ? half : kw, g);
         }
+      // m need not be the largest score, only near enough that the sums stay in range: a tile whose sums are below 2^80 is added as it is
+      bool rescale = __any(m[0] == -INFINITY || m[1] == -INFINITY);
+      if (!rescale) {
+        float sum[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = 0.f, y = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2 / KW; ++half)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              x += __builtin_amdgcn_exp2f(fmaf(s[half][i][r], a.c, -m[i]));
+              y += __builtin_amdgcn_exp2f(fmaf(s[half][i][r + 1], a.c, -m[i]));
+            }
+          sum[i] = x + y;
+        }
+        rescale = __any(!(fmaxf(sum[0], sum[1]) <= 0x1p80f));
+        if (!rescale) {
+          l[0] += sum[0];
+          l[1] += sum[1];
+        }
+      }
+      if (rescale) {
+#pragma unroll
+        for (int half = 0; half < 2 / KW; ++half)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) add_stats(s[half][i], a.c, m[i], l[i]);
       }
     }
     t = tn;
