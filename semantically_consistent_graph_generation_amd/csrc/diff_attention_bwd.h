@@ -589,9 +589,14 @@ int launch_dkv(const Args& a, hipStream_t st) {
 
 template <class T, int DP, int DVP>
 int launch_bwd(const Args& a, hipStream_t st) {
-  const bool few_q = (long long)a.B * a.H * ((a.N + 127) / 128) < 512;
-  if (const int rc = a.dq_splits > 1 ? launch_dq_split<T, DP, DVP>(a, st) : few_q ? launch_dq<T, DP, DVP, 2, 0>(a, st) : launch_dq<T, DP, DVP, 1, 0>(a, st))
-    return rc;
+  // In 32 bits above d = 32 a wave with all of a tile's keys keeps registers in memory: two share them at every size (2048 workgroups of 128
+  // queries, training pass: d = 64, dv = 128 21.0 -> 15.3 ms, d = 48, dv = 96 13.0 -> 11.1; d = 32 would lose, 5.6 -> 6.2).
+  constexpr bool SHARED = Type<T>::planes == 3 && DP > 32;
+  int rc;
+  if (a.dq_splits > 1) rc = launch_dq_split<T, DP, DVP>(a, st);
+  else if (SHARED || few_queries(a)) rc = launch_dq<T, DP, DVP, 2, 0>(a, st);
+  else rc = launch_dq<T, DP, DVP, SHARED ? 2 : 1, 0>(a, st);
+  if (rc) return rc;
   if constexpr (DkvShape<T, DP, DVP>::APART) {
     if (const int rc = launch_dkv<T, DP, DVP, 1>(a, st)) return rc;
     if (const int rc = launch_dkv<T, DP, DVP, 2>(a, st)) return rc;

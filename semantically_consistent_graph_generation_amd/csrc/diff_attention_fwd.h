@@ -450,10 +450,17 @@ int launch_split(const Args& a, hipStream_t st) {
   return 0;
 }
 
+// Few workgroups (of 128 queries): half as many queries in each, the keys of a tile shared by two waves, so that a workgroup's chain of tiles is
+// shorter.  It pays while the halves leave no CU with more than three; a causal grid, whose longest chain is its time, gains up to two
+// workgroups per CU.  Measured, one wave / two, d = 64, dv = 128, bf16, 4096 tokens: 256 workgroups 192 / 170 us, 384 262 / 271 (d = 32: 199 / 162),
+// 448 265 / 322; causal 256 198 / 140, 480 269 / 261; 512 of 2048 tokens 142 / 132, 768 169 / 183.
+inline bool few_queries(const Args& a) {
+  return (long long)a.B * a.H * (((long long)a.N + 127) / 128) <= (a.causal ? 512 : 384);
+}
+
 template <class T>
 int run_forward(const Args& a, hipStream_t st) {
-  // few workgroups: half as many queries in each, the keys of a tile shared by two waves
-  const bool few = (long long)a.B * a.H * ((a.N + 127) / 128) < 512;
+  const bool few = few_queries(a);
 #define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return few ? launch_fwd<T, DP, DVP, 2>(a, st) : launch_fwd<T, DP, DVP, 1>(a, st);
   SCGG_DIFF_WIDTHS(SCGG_X)
 #undef SCGG_X
