@@ -48,6 +48,7 @@ struct Args {
   int B, N, M, H, Hkv, d, dv_w, causal;
   int splits, split_tiles;        // forward: workgroups along the keys and the tiles each of them takes; dkv_kernel: along the queries
   int dq_splits;                  // dq_kernel: workgroups along the keys
+  bool fine;                      // 16 bits: A and dS in two terms
 };
 
 // ------------------------------------------------------------------------------------------------ element types
@@ -154,6 +155,26 @@ __device__ __forceinline__ Frag<Type<T>::planes> pack8(const float* x) {
     for (int p = 0; p < Type<T>::planes; ++p) f.p[p][i] = w[p];
   }
   return f;
+}
+
+// What pack8 left of x: x - f, rounded in turn.  From the packed words: a conversion of x for itself may be fused with the product that x comes from,
+// and then rounds a value near a tie to the other side now and then (fp16), a whole step off.
+template <class T>
+__device__ __forceinline__ Frag<Type<T>::planes> rest8(const float* x, const Frag<Type<T>::planes>& f) {
+  if constexpr (Type<T>::planes == 1) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned w = f.p[0][i];
+      const t2 h = __builtin_bit_cast(t2, w);
+      q[2 * i] = x[2 * i] - (float)h[0];
+      q[2 * i + 1] = x[2 * i + 1] - (float)h[1];
+    }
+    return pack8<T>(q);
+  } else {
+    return f;                      // nothing is left
+  }
 }
 
 // Loads of a tile go through a buffer descriptor: a 64-bit base in scalar registers for the tile, a 32-bit byte offset per lane, and

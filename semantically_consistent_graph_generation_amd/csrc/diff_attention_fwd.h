@@ -57,7 +57,7 @@ struct FwdShape {
   static constexpr int MIN_BLOCKS = P == 3 && DP > 32 ? 1 : 2;
 };
 
-template <class T, int DP, int DVP, int KW>
+template <class T, int DP, int DVP, int KW, bool FINE>
 __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void fwd_kernel(Args a) {
   typedef FwdShape<T, DP, DVP> S;
   typedef typename S::KTile KTile;
@@ -228,9 +228,13 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
           p[r] = fmaf(-lam, p2(s2[r], a.c), p1(s1[r], a.c));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const Frag<P> pf = pack8<T>(p + 8 * u);
+          const Frag<P> pf = pack8<T>(p + 8 * u), rest = FINE ? rest8<T>(p + 8 * u, pf) : pf;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) accumulate<T>(o[i], VTile::cols(vt, 32 * hh + 16 * u, 32 * i, lane, DVP), pf);
+          for (int i = 0; i < NV; ++i) {
+            const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, 32 * i, lane, DVP);
+            if (FINE) accumulate<T>(o[i], vf, rest);
+            accumulate<T>(o[i], vf, pf);
+          }
         }
       }
     }
@@ -348,14 +352,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const Frag<P> pf = pack8<T>(p + 8 * u);
-      Frag<P> rest = pf;
-      if constexpr (P == 1) {
-        float q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = p[8 * u + j] - (float)(T)p[8 * u + j];
-        rest = pack8<T>(q);
-      }
+      const Frag<P> pf = pack8<T>(p + 8 * u), rest = P == 1 ? rest8<T>(p + 8 * u, pf) : pf;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, 32 * j, lane, DVP);
@@ -427,14 +424,14 @@ __global__ __launch_bounds__(THREADS) void split_join(Args a) {
   store4<T>(static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w + c, v[0], v[1], v[2], v[3]);
 }
 
-template <class T, int DP, int DVP, int KW>
+template <class T, int DP, int DVP, int KW, bool FINE>
 int launch_fwd(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW, FINE>), S::LDS)) return -2;
   const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
   if (blocks > 0x7fffffffLL) return -3;
-  hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW, FINE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
 
@@ -461,7 +458,10 @@ inline bool few_queries(const Args& a) {
 template <class T>
 int run_forward(const Args& a, hipStream_t st) {
   const bool few = few_queries(a);
-#define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return few ? launch_fwd<T, DP, DVP, 2>(a, st) : launch_fwd<T, DP, DVP, 1>(a, st);
+  constexpr bool HALF = Type<T>::planes == 1;
+#define SCGG_X(DP, DVP) \
+  if (a.d <= DP && a.dv_w <= DVP) \
+    return HALF && a.fine ? launch_fwd<T, DP, DVP, 2, HALF>(a, st) : few ? launch_fwd<T, DP, DVP, 2, false>(a, st) : launch_fwd<T, DP, DVP, 1, false>(a, st);
   SCGG_DIFF_WIDTHS(SCGG_X)
 #undef SCGG_X
   return -1;

@@ -52,12 +52,13 @@ def mask_of(kind, B, M, g):
     return keep
 
 
-def reference(q, k, v, lam, dout, mask, causal, scale=None):
-    """Values and tolerances of out, dq, dk, dv, dlam."""
+def reference(q, k, v, lam, dout, mask, causal, scale=None, terms=1):
+    """Values and tolerances of out, dq, dk, dv, dlam; A and dS in `terms` terms: they are off by h^terms, and the sums have as many products more."""
     B, N, H2, d = q.shape
     M, H, Hkv, dv_w = k.shape[1], H2 // 2, v.shape[2], v.shape[3]
     h = torch.finfo(q.dtype).eps / 2
-    ho = 0.0 if q.dtype == torch.float32 else h
+    half = q.dtype == torch.float16
+    ho = 0.0 if q.dtype == torch.float32 else h ** terms
     group = H // Hkv
     scale = d ** -0.5 if scale is None else scale
     q, k, v, lam, dout = (t.detach().double() for t in (q, k, v, lam, dout))
@@ -75,15 +76,15 @@ def reference(q, k, v, lam, dout, mask, causal, scale=None):
     dp = ein("bnhe,bmhe->bhnm", dout, V)
     D = ein("bnhe,bmhe->bhnm", dout.abs(), V.abs())
     smax = float((ein("bnhid,bmhid->bhinm", Q.abs(), K.abs()) * scale * see[:, None, None]).amax()) if M * N else 0.0
-    C, C2, S = 6 * d / 16 + 16, 6 * dv_w / 16 + 16, M / 16 + 32
+    C, C2, S = 6 * d / 16 + 16, 6 * dv_w / 16 + 16, terms * M / 16 + 32
     E = 2 * (C * U * smax + 8 * U * (1 + smax)) + 64 * U
     low_a = low_s = 2.0 ** -125
-    if ho == 2.0 ** -11 and dp.numel():
+    if half and dp.numel():
         low_a = 2.0 ** -38 * max(1.0, float(lam.abs().max()))
         low_s = 2 * low_a * float(dp.abs().max())
     seen = see[:, None].double().expand_as(a)
     tol_out = low_a * ein("bhnm,bmhe->bnhe", seen, V.abs()) + ho * ein("bhnm,bmhe->bnhe", a.abs(), V.abs()) + (E + S * U) * ein("bhnm,bmhe->bnhe", both, V.abs()) + h * out.abs()
-    SN = N * group / 16 + 32
+    SN = terms * N * group / 16 + 32
     tol_dv = low_a * ein("bhnm,bnhe->bmhe", seen, dout.abs()) + ho * ein("bhnm,bnhe->bmhe", a.abs(), dout.abs()) + (E + SN * U) * ein("bhnm,bnhe->bmhe", both, dout.abs())
     dq, dk, tq, tk = [], [], [], []
     dlam = tol_lam = None
@@ -347,3 +348,30 @@ def test_a_layer_of_the_three_operators():
     want = layer(*wide, False)
     for a, b in zip((out,) + grads, (want,) + torch.autograd.grad(want, wide, dout.double())):
         assert float((a.detach().double() - b.detach()).abs().max()) < 2 ** -13 * float(b.detach().abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", CASES + [(1, 1, 188, 1, 1, 40, 80, "ragged", False), (3, 8, 8, 6, 3, 32, 64, "none", False),
+                                          (1, 60, 8000, 1, 1, 64, 128, "none", False)], ids=str)
+def test_small_problems_round_outputs_only(case, dtype):
+    """Up to 2^24 pairs of tokens the entries of A and dS are taken in two terms: h^2 in the place of h, so the output's own rounding is what is left."""
+    B, N, M, H, Hkv, d, dv, kind, causal = case
+    assert B * H * N * M <= 2 ** 24
+    q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, 3 * N + M + d)
+    mask = mask_of(kind, B, M, g)
+    check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal), reference(q, k, v, lam, dout, mask, causal, terms=2))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", [
+    (8, 201, 190, 64, 32, 64, 128, "none", True), (8, 190, 201, 64, 32, 48, 96, "ragged", False), (8, 201, 190, 64, 64, 64, 64, "random", False),
+    (8, 201, 190, 64, 32, 32, 32, "none", True), (16, 201, 190, 32, 16, 32, 64, "ragged", False),        # 128 queries to a workgroup
+    (1, 2100, 2100, 4, 2, 64, 128, "none", True), (1, 2100, 2100, 4, 4, 32, 64, "none", False),          # 64; causal: the dQ kernel's keys in two
+    (1, 1000, 4300, 4, 4, 48, 96, "ragged", False), (1, 1100, 8000, 2, 2, 64, 64, "rare", False)], ids=str)  # keys split
+def test_large_problems(case, dtype):
+    """Above 2^24 pairs of tokens: one term, as the tolerances above say."""
+    B, N, M, H, Hkv, d, dv, kind, causal = case
+    assert B * H * N * M > 2 ** 24
+    q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, N + M + d)
+    mask = mask_of(kind, B, M, g)
+    check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal), reference(q, k, v, lam, dout, mask, causal))
