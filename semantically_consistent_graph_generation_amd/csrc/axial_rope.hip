@@ -10,9 +10,9 @@
 // and sines of the tile, each once for all heads of q and k: positions reach 1e6 and beyond, so the angle is a product in
 // 64 bits, reduced to an eighth of a turn there, and only then rounded to 32.  Then the heads stream through, 16 B per load: a
 // head belongs to a power of two of lanes that hold whole pairs, so the rotation needs no exchange and the norm one butterfly.
-// In the backward of a norm a workgroup belongs to q or to
-// k, so that a lane has one side's weights and sums (157 -> 142 registers; 281 -> 258 us for 4 x 16384 tokens of 20 bf16 heads of 128); elsewhere
-// it takes both, and the cosines are formed once (21 against 25 us for 27648 tokens of 16 heads of 64).  Statistics and products are 32-bit, each output is rounded once.  The weight gradients are summed per lane (a lane keeps
+// In the backward of a norm a workgroup belongs to q or to k, so that a lane has one side's weights and sums (281 -> 258 us for 4 x 16384 tokens of
+// 20 bf16 heads of 128; 252 now, the forward 162, together 1.68 GB at 4.0 TB/s); elsewhere it takes both, and the cosines are formed once (21
+// against 25 us for 27648 tokens of 16 heads of 64).  Statistics and products are 32-bit, each output is rounded once.  The weight gradients are summed per lane (a lane keeps
 // its channels), per workgroup through LDS, and over the workgroups by a second kernel in a fixed order: no atomics, equal
 // calls give equal bits.
 #include <hip/hip_runtime.h>

@@ -8,7 +8,7 @@
 // products over 16 slots each (the slots' order is the rows' order, so the other operand is read in that order).
 //
 // Types: bf16 and fp16 multiply as they are.  fp32 is split exactly into three bf16 terms (h + m + l) and a product is the six
-// leading partial products, which keeps fp32's accuracy at 2.7 times the rate of the fp32 matrix instructions.  A tile in LDS has a plane per
+// leading partial products, which keeps fp32's accuracy at up to 2.7 times the rate of the fp32 matrix instructions (peaks: 2500 / 6 against 157 TFLOP/s).  A tile in LDS has a plane per
 // term, so the kernels are the same for all types.
 //
 // Tiles in LDS: 64 rows (keys, or queries in the dK / dV kernel), read row-wise (b128) and transposed (tr_b64).

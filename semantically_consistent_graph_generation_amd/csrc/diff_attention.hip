@@ -12,7 +12,8 @@ namespace {
 // 649 / 770.
 constexpr double FINE_PAIRS = 1 << 24;
 constexpr int SPLIT_MIN_TILES = 4;     // keys of a split workgroup at least: 4 tiles of 64
-constexpr int SPLIT_GROUPS = 1024;     // workgroups that keep the memory busy: 4 on each of 256 CUs
+constexpr int SPLIT_GROUPS = 1024;     // workgroups that keep the memory busy: 4 on each of 256 CUs (512, 1024, 2048, 4096: one query x 32768 keys
+                                       // of 16 x 4 key heads 202, 208, 206, 225 us; 65536 keys of 4 x 4 109, 108, 114, 137)
 
 // dlambda[h] = - sum over sequences and queries of delta_2, in a fixed order: 256 lanes, each a stretch, then a tree
 __global__ __launch_bounds__(256) void dlambda_kernel(const float* __restrict__ delta, float* __restrict__ out, int B, int H, int N) {
@@ -86,7 +87,9 @@ Args make(const scgg_diff_attention_args* p) {
 }
 
 // Keys split over workgroups (0: not): where the queries give the other kernel less than one workgroup (of 64) to every second CU, and
-// there are keys to split.  Such a kernel is one long chain of tiles on a few CUs.
+// there are keys to split.  Such a kernel is one long chain of tiles on a few CUs.  Split / not,
+// us a call, d = 64, dv = 128, bf16: 60 queries x 8000 keys 25 / 242; 8 heads of 512 x 4096 68 / 130; of 900 x 4096 (120 workgroups) 91 to 98 / 128 to 131;
+// one query of 16 heads on 4 x 64 x 2048 keys 55 / 253.
 void plan_split(Args& a) {
   const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32);
   a.splits = 0;
@@ -102,7 +105,8 @@ size_t part_bytes(const Args& a) {
   return a.splits == 0 ? 0 : (size_t)a.B * a.H * a.N * 2 * a.splits * (2 * a.dv_w + 4) * sizeof(float);
 }
 // Queries split over workgroups in the dK / dV kernel: where the keys alone give fewer than two workgroups to each CU, and there are tiles to
-// split.  Each split writes its sums in 32 bits and they are read again, so there are four at most.
+// split.  Each split writes its sums in 32 bits and they are read again, so there are four at most.  Training pass with 1, 2, 4, 8 splits allowed:
+// 4096 causal, 8 heads on 4, 905, 622, 490, 490 us; not causal 1002, 721, 651, 652; 16 heads of 2048 375, 360, 360, 361.
 void plan_dkv(Args& a) {
   const long long blocks = (long long)a.B * a.Hkv * ((a.M + 127) / 128), tiles = (long long)((a.N + TILE - 1) / TILE) * (a.H / a.Hkv);
   long long s = blocks > 0 ? 512 / blocks : 1;
@@ -112,7 +116,7 @@ void plan_dkv(Args& a) {
 }
 // Keys split over workgroups in the dQ kernel: as in the forward, where the queries (64 to a workgroup) fill less than half of the GPU.  The
 // splits' dQ and the sweeps' second launch cost about as much as eight tiles.  Causal grids of up to two workgroups per CU are split in two: all of
-// them run at once, so the longest is the time, and halving it is worth the join (4096 causal: 199 -> 180 us).
+// them run at once, so the longest is the time, and halving it is worth the join (4096 causal, 8 heads on 4, training pass: 513 -> 490 us).
 void plan_dq(Args& a) {
   const long long blocks = (long long)a.B * a.H * ((a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
   long long s = blocks > 0 && blocks < 128 ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;

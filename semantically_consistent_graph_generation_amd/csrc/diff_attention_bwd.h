@@ -4,7 +4,11 @@
 //   delta_i = sum_j P_i dP,  dQ_i = scale dS_i K_i,  dK_i = scale dS_i^T Q_i,  dlambda = - sum delta_2
 //
 // Two kernels, each of which owns what it writes (no atomics): one over queries for delta and dQ, one over keys for dK and dV.
-// delta comes from a sweep of its own, formed in 32 bits: dlambda is its sum, and dS a difference with it.
+// delta comes from a sweep of its own, formed in 32 bits: dlambda is its sum, and dS a difference with it (dO . out would save the sweep, but out
+// is rounded, and the gradient of a row with one key would not be zero).
+// Bound: the vector and the matrix unit.  32 heads of 4096 x 4096, d = 64, dv = 128, bf16, mean of a trace (the forward 643 us): dQ 870 us, vector
+// instructions issue in 57 % of the cycles, the matrix unit is busy in 42; dK 582 us, 47 and 37 %; dV 440 us, 43 and 32 %.  4096 causal, 8 heads on 4:
+// dQ 73 + 97 with 5 + 8 for its joins, dK 116, dV 86, join 12, forward 155.
 #pragma once
 #include "diff_attention_fwd.h"
 
