@@ -267,7 +267,7 @@ def _diff_forward(q, k, v, lam, mask, cfg, with_stats=False):
     a = _diff_args(q, k, v, lam, mask, cfg)
     out = torch.empty(q.shape[0], q.shape[1], a.H, a.dv, dtype=q.dtype, device=q.device)
     a.out = out.data_ptr()
-    stats = torch.empty(a.B, a.H, 2, a.N, 2, device=q.device) if with_stats else None
+    stats = torch.empty(a.B, a.H, 2, a.N, 2, dtype=torch.float32, device=q.device) if with_stats else None
     a.stats = stats.data_ptr() if with_stats else None
     nbytes = L.scgg_diff_attention_forward_workspace_bytes(C.byref(a))
     ws = _workspace(nbytes, q.device)
@@ -327,7 +327,7 @@ def diff_attention(q, k, v, lam, key_mask=None, causal=False, scale=None):
     if d < 8 or dv < 8 or d % 8 or dv % 8 or d > 64 or dv > 128:
         _fail(what, f"d = {d}, dv = {dv}: multiples of 8 with d <= 64 and dv <= 128 are supported")
     if not isinstance(lam, torch.Tensor):
-        lam = torch.full((H,), float(lam), device=q.device)
+        lam = torch.full((H,), float(lam), dtype=torch.float32, device=q.device)
     if lam.dtype != torch.float32 or lam.device != q.device or tuple(lam.shape) not in ((), (1,), (H,)):
         _fail(what, f"lam has to be float32, [{H}] or a scalar, on {q.device}")
     lam = lam.expand(H).contiguous()

@@ -148,3 +148,24 @@ def test_sit_refuses_heads_that_do_not_pair():
     for kw in (dict(num_heads=3), dict(num_heads=5), dict(hidden_size=768, num_heads=4), dict(hidden_size=72, num_heads=6), dict(attention="other")):
         with pytest.raises(_lib.ScggError, match="SiT"):
             SiT(**{"attention": "differential", **kw})
+
+
+def test_default_dtype_is_not_used(monkeypatch):
+    """A number for lam, and the statistics that the kernels write in 32 bits, whatever torch's default type is."""
+    made = []
+    for name in ("full", "empty"):
+        def kept(*a, _of=getattr(torch, name), **kw):
+            made.append(_of(*a, **kw))
+            return made[-1]
+        monkeypatch.setattr(A.torch, name, kept)
+    monkeypatch.setattr(A, "_call", lambda *a: 0)
+    monkeypatch.setattr(A, "_check_device", lambda *a: None)
+    q, k, v = (torch.zeros(1, 3, h, 8, dtype=torch.bfloat16) for h in (2, 2, 1))
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        A.diff_attention(q.requires_grad_(), k, v, 0.5)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    lam, out, stats = made[:3]
+    assert lam.dtype == torch.float32 and out.dtype == torch.bfloat16
+    assert stats.dtype == torch.float32 and stats.numel() == 2 * 3 * 2

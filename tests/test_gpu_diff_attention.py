@@ -375,3 +375,14 @@ def test_large_problems(case, dtype):
     q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, N + M + d)
     mask = mask_of(kind, B, M, g)
     check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal), reference(q, k, v, lam, dout, mask, causal))
+
+
+def test_default_dtype_changes_nothing():
+    q, k, v, lam, dout, g = make(2, 70, 90, 2, 1, 32, 64, "bf16", 20)
+    want = run_all(q, k, v, lam, dout), op()(q, k, v, 0.25)
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = run_all(q, k, v, lam, dout), op()(q, k, v, 0.25)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(a, b) for a, b in zip(want[0], got[0])) and torch.equal(want[1], got[1])
