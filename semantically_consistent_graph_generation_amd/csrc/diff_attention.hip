@@ -44,11 +44,13 @@ int check(const scgg_diff_attention_args* p, const char* what) {
   if (p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0) return fail("%s: %d heads on %d key heads", what, p->H, p->Hkv);
   if (p->d < 8 || p->dv < 8 || p->d % 8 != 0 || p->dv % 8 != 0 || p->d > 64 || p->dv > 128)
     return fail("%s: d = %d, dv = %d: multiples of 8 with d <= 64 and dv <= 128 are supported", what, p->d, p->dv);
-  if (!(p->scale > 0.f) || !isfinite(p->scale)) return fail("%s: scale has to be positive and finite", what);
+  if (!(p->scale > 0.f) || !isfinite(p->scale * 1.44269504088896340736f)) return fail("%s: scale has to be positive and, times log2(e), finite", what);
   if (p->N > 0x7fffffff - 256 || p->M > 0x7fffffff - 256) return fail("%s: too many tokens", what);
   if ((long long)p->B * p->H > 0x7fffffff || (long long)p->B * p->N * p->H > 0x7fffffffLL * 32) return fail("%s: too many rows", what);
   return 0;
 }
+
+bool aligned16(const void* base) { return (reinterpret_cast<uintptr_t>(base) & 15) == 0; }
 
 bool aligned(const scgg_diff_attention_args* p, const void* base, int64_t sb, int64_t sn, int64_t sh) {
   const int64_t size = p->dtype == SCGG_F32 ? 4 : 2;
@@ -172,6 +174,7 @@ extern "C" int scgg_diff_attention_forward(const scgg_diff_attention_args* p, vo
   if (check(p, what) || check_inputs(p, what)) return -1;
   if (p->B == 0 || p->N == 0) return 0;
   if (!p->out) return fail("%s: null output", what);
+  if (!aligned16(p->out) || !aligned16(p->stats)) return fail("%s: out and stats have to be aligned to 16 bytes", what);
   Args a = make(p);
   plan_split(a);
   const size_t need = part_bytes(a);
@@ -192,6 +195,8 @@ extern "C" int scgg_diff_attention_backward(const scgg_diff_attention_args* p, v
   if (queries && !aligned(p, p->dout, p->dout_stride_b, p->dout_stride_n, p->dout_stride_h))
     return fail("%s: base and strides of dout have to be multiples of 16 bytes", what);
   if (queries && !near(p, p->dout_stride_n, 0, p->dv)) return fail("%s: rows of dout have to lie less than 2 GiB / 64 apart", what);
+  if (!aligned16(p->dq) || !aligned16(p->dk) || !aligned16(p->dv_out) || !aligned16(p->stats))
+    return fail("%s: dq, dk, dv_out and stats have to be aligned to 16 bytes", what);
   Args a = make(p);
   const size_t need = backward_bytes(a);
   if (check_workspace(need, workspace, workspace_bytes, what)) return -1;

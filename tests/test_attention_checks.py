@@ -169,3 +169,14 @@ def test_default_dtype_is_not_used(monkeypatch):
     lam, out, stats = made[:3]
     assert lam.dtype == torch.float32 and out.dtype == torch.bfloat16
     assert stats.dtype == torch.float32 and stats.numel() == 2 * 3 * 2
+
+
+def test_diff_c_entry_refuses_outputs_off_the_grid_and_scales_out_of_range():
+    """The kernels store 8 or 16 bytes at once, and take scale log2(e) in 32 bits."""
+    L = _lib.lib()
+    for n in ("out", "stats"):
+        assert L.scgg_diff_attention_forward(C.byref(diff_args(**{n: 4104})), None, 0, None) != 0 and "aligned" in L.scgg_last_error().decode()
+    for n in ("dq", "dk", "dv_out", "stats"):
+        assert L.scgg_diff_attention_backward(C.byref(diff_args(**{n: 4104})), 4096, 1 << 30, None) != 0 and "aligned" in L.scgg_last_error().decode()
+    a = diff_args(scale=3e38)
+    assert L.scgg_diff_attention_forward(C.byref(a), None, 0, None) != 0 and "scale" in L.scgg_last_error().decode()
