@@ -166,7 +166,8 @@ class SiT(nn.Module):
         return self._forward_engine(x, t, padding_mask)
 
     def _forward_differential(self, x, t, padding_mask):
-        x, mask = x.float(), padding_mask.to(torch.bool)
+        mask = padding_mask.to(torch.bool)
+        x = x.float().masked_fill(~mask[..., None], 0.0)          # whatever padded rows hold: 0 times a NaN would reach the weights' gradients
         dim = self.hidden_size
         half = self.t_embedder.mlp[0].in_features // 2
         arg = t.float()[:, None] * torch.exp(torch.arange(half, device=x.device) * (-math.log(10000.0) / half))
@@ -190,7 +191,8 @@ class SiT(nn.Module):
         beta = torch.linspace(self.beta_start, self.beta_end, self.noise_steps)
         alpha = 1.0 - beta
         alpha_hat = torch.cumprod(alpha, 0)
-        x, mask = x_T.detach().float().contiguous(), node_mask.to(torch.bool)
+        mask = node_mask.to(torch.bool)
+        x = x_T.detach().float().masked_fill(~mask[..., None], 0.0).contiguous()
         B, n = x.shape[:2]
         z = torch.empty_like(x)
         for k, i in enumerate(range(self.noise_steps - 1, 0, -1)):
@@ -203,7 +205,7 @@ class SiT(nn.Module):
                 if noise is None and z.numel():
                     _lib.check(_lib.lib().scgg_philox_normal_rows(_lib.ptr(z), B, n, seed, graph_id_base, i, _lib.stream_ptr()), "philox_normal_rows")
                 x = x + math.sqrt(be) * (z if noise is None else noise[k].float())
-        return x * mask[..., None]
+        return x.masked_fill(~mask[..., None], 0.0)
 
     @torch.no_grad()
     def _forward_engine(self, x, t, padding_mask):

@@ -79,3 +79,24 @@ def test_coordinate_model_and_default():
     out = cm.sample(torch.randn(2, 7, 3, device="cuda"), m, seed=1)
     assert out.shape == (2, 7, 3) and torch.isfinite(out).all()
     assert not any("norm" in k or "lambda" in k for k in SiT().state_dict())
+
+
+def test_padded_rows_may_hold_anything():
+    """Output, sampler and gradients with NaN and infinities in the padded rows are those with zeros there, bit for bit, and 0 on them."""
+    model = build()
+    m = fx.ragged_mask([12, 5, 1]).cuda()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(*m.shape, 3, generator=g, device="cuda").masked_fill(~m[..., None], 0.0)
+    t = torch.tensor([999, 500, 3], device="cuda")
+    do = torch.randn(x.shape, generator=g, device="cuda")
+    params = list(model.parameters())
+
+    def run(x):
+        x = x.clone().requires_grad_()
+        out = model(x, t, m)
+        return (out.detach(),) + torch.autograd.grad(out, [x] + params, do)
+    dirty = torch.where(m[..., None], x, torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda"))
+    clean, got = run(x), run(dirty)
+    assert all(torch.equal(a, b) for a, b in zip(clean, got)) and torch.isfinite(got[0]).all() and not got[0][~m].any() and not got[1][~m].any()
+    chain = [model._sample_differential(y, m, 3, None, 7, 0) for y in (x, dirty)]
+    assert torch.equal(*chain) and not chain[1][~m].any()
