@@ -88,14 +88,16 @@ Args make(const scgg_diff_attention_args* p) {
   return a;
 }
 
-// Keys split over workgroups (0: not): where the queries give the other kernel less than one workgroup (of 64) to every second CU, and
-// there are keys to split.  Such a kernel is one long chain of tiles on a few CUs.  Split / not,
-// us a call, d = 64, dv = 128, bf16: 60 queries x 8000 keys 25 / 242; 8 heads of 512 x 4096 68 / 130; of 900 x 4096 (120 workgroups) 91 to 98 / 128 to 131;
-// one query of 16 heads on 4 x 64 x 2048 keys 55 / 253.
+// Keys split over workgroups (0: not): for up to 32 rows of a key head, and where the queries give the other kernel, one long chain of tiles on a part of
+// the CUs, few workgroups (of 64).  The split kernel does more work per tile and its join costs by the row, so the more workgroups, the more keys it
+// takes: up to 4 workgroups per tile of keys, and 160.  us a call not split / split, 8 heads, d = 64, dv = 128, bf16: 10 tiles, 32 workgroups 28 / 25, 64
+// 28 / 30; 16 tiles, 64 40 / 34, 96 40 / 47, 120 40 / 52; 32 tiles, 128 73 / 70, 160 68 / 80; 64 tiles, 128 129 / 102, 160 129 / 119, 192 129 / 132;
+// 256 tiles, 160 499 / 343.  One query of 16 heads on 4 x 64 x 2048 keys 253 / 55; 60 queries x 8000 keys 242 / 25.
 void plan_split(Args& a) {
   const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32);
+  const long long others = (long long)a.B * a.H * (((long long)a.N + 63) / 64), most = tiles < 40 ? 4 * tiles : 160;
   a.splits = 0;
-  if ((rows > 32 && (long long)a.B * a.H * ((a.N + 63) / 64) >= 128) || tiles < 2 * SPLIT_MIN_TILES || blocks == 0) return;
+  if ((rows > 32 && others > most) || tiles < 2 * SPLIT_MIN_TILES || blocks == 0) return;
   long long s = SPLIT_GROUPS / blocks;
   if (s > tiles / SPLIT_MIN_TILES) s = tiles / SPLIT_MIN_TILES;
   if (s < 1) s = 1;
@@ -116,12 +118,14 @@ void plan_dkv(Args& a) {
   if (s > tiles / 4) s = tiles / 4;
   a.splits = s < 1 ? 1 : (int)s;
 }
-// Keys split over workgroups in the dQ kernel: as in the forward, where the queries (64 to a workgroup) fill less than half of the GPU.  The
-// splits' dQ and the sweeps' second launch cost about as much as eight tiles.  Causal grids of up to two workgroups per CU are split in two: all of
-// them run at once, so the longest is the time, and halving it is worth the join (4096 causal, 8 heads on 4, training pass: 513 -> 490 us).
+// Keys split over workgroups in the dQ kernel, where the queries (64 to a workgroup) fill about half of the GPU or less.  The splits' dQ and the
+// sweeps' second launch cost about as much as eight tiles.  Training pass, not split / split, 8 heads: 128 workgroups, 16 tiles, fp32, d = 64 418 / 345 us (bf16
+// 162 / 169), 64 tiles, bf16 382 / 300; 160 workgroups, 16 tiles, fp32 436 / 463, 32 tiles 837 / 755 (bf16 225 / 202).  Causal grids of up to two workgroups
+// per CU are split in two: all of them run at once, so the longest is the time, and halving it is worth the join (4096 causal, 8 heads on 4, training pass:
+// 513 -> 490 us).
 void plan_dq(Args& a) {
-  const long long blocks = (long long)a.B * a.H * ((a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
-  long long s = blocks > 0 && blocks < 128 ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;
+  const long long blocks = (long long)a.B * a.H * (((long long)a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
+  long long s = blocks > 0 && blocks <= (tiles < 32 ? 128 : 160) ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;
   if (s > 16) s = 16;
   if (s > tiles / 8) s = tiles / 8;
   a.dq_splits = s < 1 ? 1 : (int)s;

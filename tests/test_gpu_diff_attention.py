@@ -386,3 +386,14 @@ def test_default_dtype_changes_nothing():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(a, b) for a, b in zip(want[0], got[0])) and torch.equal(want[1], got[1])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("case", [(1, 500, 1000, 8, 8, 32, 64, False), (1, 600, 1000, 8, 4, 32, 64, False), (1, 1250, 2570, 8, 8, 64, 128, False),
+                                  (1, 1300, 2570, 8, 4, 48, 96, True), (1, 1250, 2000, 8, 8, 32, 32, False), (1, 1000, 700, 8, 8, 64, 64, True)], ids=str)
+def test_at_the_bounds_of_the_splits(case, dtype):
+    """Both sides of the rules that split the keys: workgroups against tiles of keys, in the forward and in the dQ kernel."""
+    B, N, M, H, Hkv, d, dv, causal = case
+    q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, N + M)
+    mask = mask_of("random", B, M, g)
+    check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal), reference(q, k, v, lam, dout, mask, causal))
