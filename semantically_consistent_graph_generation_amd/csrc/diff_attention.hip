@@ -6,11 +6,6 @@ namespace scgg {
 namespace diffattn {
 namespace {
 
-// 16 bits: up to so many pairs (heads x queries x keys) the entries of A and dS go into their product in two terms, rounded and rest.  Rounded once
-// they add about as much error as the output's rounding (1.41 of it together), and where few rows or keys are summed more (1.67 seen).  bf16, forward and
-// training pass, one term / two: 4.2 M 34 / 33, 172 / 173 us; 8.4 M 38 / 41, 165 / 164; 10 M 45 / 48, 155 / 169; 34 M 69 / 74, 247 / 275; 134 M 167 / 190,
-// 649 / 770.
-constexpr double FINE_PAIRS = 1 << 24;
 constexpr int SPLIT_MIN_TILES = 4;     // keys of a split workgroup at least: 4 tiles of 64
 constexpr int SPLIT_GROUPS = 1024;     // workgroups that keep the memory busy: 4 on each of 256 CUs (512, 1024, 2048, 4096: one query x 32768 keys
                                        // of 16 x 4 key heads 202, 208, 206, 225 us; 65536 keys of 4 x 4 109, 108, 114, 137)
@@ -84,7 +79,6 @@ Args make(const scgg_diff_attention_args* p) {
   a.gb = p->dout_stride_b; a.gn = p->dout_stride_n; a.gh = p->dout_stride_h; a.mb = p->mask_stride_b;
   a.scale = p->scale; a.c = p->scale * 1.44269504088896340736f;
   a.B = p->B; a.N = p->N; a.M = p->M; a.H = p->H; a.Hkv = p->Hkv; a.d = p->d; a.dv_w = p->dv; a.causal = p->causal != 0;
-  a.fine = p->dtype != SCGG_F32 && (double)a.B * a.H * a.N * a.M <= FINE_PAIRS;
   return a;
 }
 

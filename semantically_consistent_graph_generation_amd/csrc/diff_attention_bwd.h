@@ -30,7 +30,7 @@ struct DqShape {
 // delta [B,H,3,N]: delta_1, delta_2, and the largest |dP| of the query.
 // PHASE 0: both sweeps.  With few queries the keys are split over `dq_splits` workgroups, and the sweeps are launches of their own: 1 writes
 // the splits' deltas to `part` (delta_join adds them), 2 the splits' dQ in 32 bits (dq_join).
-template <class T, int DP, int DVP, int KW, int PHASE, bool FINE>
+template <class T, int DP, int DVP, int KW, int PHASE>
 __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq_kernel(Args a) {
   typedef DqShape<T, DP, DVP> S;
   typedef typename S::KTile KTile;
@@ -217,11 +217,11 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
           for (int r = 0; r < 16; ++r) ds[r] = prob[i](s[r], a.c) * fmaf(dp[r], w[i], wd[i]);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const Frag<P> df = pack8<T>(ds + 8 * u), rest = FINE ? rest8<T>(ds + 8 * u, df) : df;
+            const Frag<P> df = pack8<T>(ds + 8 * u), rest = TWO_TERMS<T> ? rest8<T>(ds + 8 * u, df) : df;
 #pragma unroll
             for (int j = 0; j < ND; ++j) {
               const Frag<P> kc = KTile::cols(kt, 32 * hh + 16 * u, i * DP + 32 * j, lane, (i + 1) * DP);
-              if (FINE) accumulate<T>(o[i][j], kc, rest);
+              if (TWO_TERMS<T>) accumulate<T>(o[i][j], kc, rest);
               accumulate<T>(o[i][j], kc, df);
             }
           }
@@ -315,7 +315,7 @@ constexpr int BK = 128;                                             // keys of a
 // Over keys: a wave keeps 32 of them (k1, k2 and v as operands, dK1, dK2 and dV as sums) and the queries of all heads that share the key
 // head stream by.  With few keys the queries are split over `splits` workgroups, whose sums go to `part` [splits][B M Hkv][2 d + dv]
 // in 32 bits and are added in order by dkv_join.  WHAT: 1 dK, 2 dV, 3 both.
-template <class T, int DP, int DVP, int WHAT, bool FINE>
+template <class T, int DP, int DVP, int WHAT>
 __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void dkv_kernel(Args a) {
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   typedef DkvShape<T, DP, DVP> S;
@@ -488,13 +488,13 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
         if (DK) {
           fs[i][0] = pack8<T>(ds);
           fs[i][1] = pack8<T>(ds + 8);
-          if (FINE) { rest_s[i][0] = rest8<T>(ds, fs[i][0]); rest_s[i][1] = rest8<T>(ds + 8, fs[i][1]); }
+          if (TWO_TERMS<T>) { rest_s[i][0] = rest8<T>(ds, fs[i][0]); rest_s[i][1] = rest8<T>(ds + 8, fs[i][1]); }
         }
       }
       if (DV) {
         fa[0] = pack8<T>(p);
         fa[1] = pack8<T>(p + 8);
-        if (FINE) { rest_a[0] = rest8<T>(p, fa[0]); rest_a[1] = rest8<T>(p + 8, fa[1]); }
+        if (TWO_TERMS<T>) { rest_a[0] = rest8<T>(p, fa[0]); rest_a[1] = rest8<T>(p + 8, fa[1]); }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
             const Frag<P> gc = GTile::cols(gt, row0, 32 * j, lane, DVP);
-            if (FINE) accumulate<T>(dv[j], gc, rest_a[u]);
+            if (TWO_TERMS<T>) accumulate<T>(dv[j], gc, rest_a[u]);
             accumulate<T>(dv[j], gc, fa[u]);
           }
         }
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
 #pragma unroll
           for (int j = 0; j < ND; ++j) {
             const Frag<P> q1 = QTile::cols(qt, row0, 32 * j, lane, DP), q2 = QTile::cols(qt, row0, DP + 32 * j, lane, 2 * DP);
-            if (FINE) {
+            if (TWO_TERMS<T>) {
               accumulate<T>(dk[0][j], q1, rest_s[0][u]);
               accumulate<T>(dk[1][j], q2, rest_s[1][u]);
             }
@@ -572,54 +572,54 @@ __global__ __launch_bounds__(256) void dkv_join(Args a, long long quads) {
   store4<T>(dst, v[0], v[1], v[2], v[3]);
 }
 
-template <class T, int DP, int DVP, int KW, int PHASE, bool FINE>
+template <class T, int DP, int DVP, int KW, int PHASE>
 int launch_dq(const Args& a, hipStream_t st) {
   typedef DqShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW, PHASE, FINE>), S::LDS)) return -2;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW, PHASE>), S::LDS)) return -2;
   const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW)) * (PHASE == 0 ? 1 : a.dq_splits);
   if (blocks > 0x7fffffffLL) return -3;
-  if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW, PHASE, FINE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW, PHASE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
 
-template <class T, int DP, int DVP, bool FINE>
+template <class T, int DP, int DVP>
 int launch_dq_split(const Args& a, hipStream_t st) {
   const long long rows = (long long)a.B * a.H * a.N, quads = rows * 2 * a.d / 4;
   if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
-  if (const int rc = launch_dq<T, DP, DVP, 2, 1, false>(a, st)) return rc;
+  if (const int rc = launch_dq<T, DP, DVP, 2, 1>(a, st)) return rc;
   hipLaunchKernelGGL(delta_join, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);
-  if (const int rc = launch_dq<T, DP, DVP, 2, 2, FINE>(a, st)) return rc;
+  if (const int rc = launch_dq<T, DP, DVP, 2, 2>(a, st)) return rc;
   hipLaunchKernelGGL((dq_join<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, quads);
   return 0;
 }
 
-template <class T, int DP, int DVP, int WHAT, bool FINE>
+template <class T, int DP, int DVP, int WHAT>
 int launch_dkv(const Args& a, hipStream_t st) {
   typedef DkvShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT, FINE>), S::lds(WHAT))) return -2;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT>), S::lds(WHAT))) return -2;
   const long long blocks = (long long)a.B * a.Hkv * ((a.M + BK - 1) / BK) * a.splits;
   if (blocks > 0x7fffffffLL) return -3;
-  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT, FINE>), dim3((unsigned)blocks), dim3(THREADS), S::lds(WHAT), st, a);
+  if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT>), dim3((unsigned)blocks), dim3(THREADS), S::lds(WHAT), st, a);
   return 0;
 }
 
-template <class T, int DP, int DVP, bool FINE>
+template <class T, int DP, int DVP>
 int launch_bwd(const Args& a, hipStream_t st) {
   // In 32 bits above d = 32 a wave with all of a tile's keys keeps registers in memory: two share them at every size (2048 workgroups of 128
   // queries, training pass: d = 64, dv = 128 21.0 -> 15.3 ms, d = 48, dv = 96 13.0 -> 11.1; d = 32 would lose, 5.6 -> 6.2).
-  constexpr bool SHARED = FINE || (Type<T>::planes == 3 && DP > 32);
+  constexpr bool SHARED = Type<T>::planes == 3 && DP > 32;
   int rc;
-  if (a.dq_splits > 1) rc = launch_dq_split<T, DP, DVP, FINE>(a, st);
-  else if (SHARED || few_queries(a)) rc = launch_dq<T, DP, DVP, 2, 0, FINE>(a, st);
-  else rc = launch_dq<T, DP, DVP, SHARED ? 2 : 1, 0, FINE>(a, st);
+  if (a.dq_splits > 1) rc = launch_dq_split<T, DP, DVP>(a, st);
+  else if (SHARED || few_queries(a)) rc = launch_dq<T, DP, DVP, 2, 0>(a, st);
+  else rc = launch_dq<T, DP, DVP, SHARED ? 2 : 1, 0>(a, st);
   if (rc) return rc;
   if constexpr (DkvShape<T, DP, DVP>::APART) {
-    if (const int rc1 = launch_dkv<T, DP, DVP, 1, FINE>(a, st)) return rc1;
-    if (const int rc2 = launch_dkv<T, DP, DVP, 2, FINE>(a, st)) return rc2;
+    if (const int rc1 = launch_dkv<T, DP, DVP, 1>(a, st)) return rc1;
+    if (const int rc2 = launch_dkv<T, DP, DVP, 2>(a, st)) return rc2;
   } else {
-    if (const int rc3 = launch_dkv<T, DP, DVP, 3, FINE>(a, st)) return rc3;
+    if (const int rc3 = launch_dkv<T, DP, DVP, 3>(a, st)) return rc3;
   }
   const long long quads = (long long)a.B * a.M * a.Hkv * (2 * a.d + a.dv_w) / 4;
   if (a.splits > 1 && quads > 0) {
@@ -631,9 +631,7 @@ int launch_bwd(const Args& a, hipStream_t st) {
 
 template <class T>
 int run_backward(const Args& a, hipStream_t st) {
-  constexpr bool HALF = Type<T>::planes == 1;
-#define SCGG_X(DP, DVP) \
-  if (a.d <= DP && a.dv_w <= DVP) return HALF && a.fine ? launch_bwd<T, DP, DVP, HALF>(a, st) : launch_bwd<T, DP, DVP, false>(a, st);
+#define SCGG_X(DP, DVP) if (a.d <= DP && a.dv_w <= DVP) return launch_bwd<T, DP, DVP>(a, st);
   SCGG_DIFF_WIDTHS(SCGG_X)
 #undef SCGG_X
   return -1;

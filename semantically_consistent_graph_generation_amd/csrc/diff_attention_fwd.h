@@ -41,7 +41,7 @@ __device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float 
 }
 
 // Two sweeps over the keys.  The first finds the maximum and the sum of both maps; the second forms A = P1 - lambda P2 in 32 bits, rounds
-// it once (FINE: in two terms, see FINE_PAIRS), and needs one product with v.  With dv = 2 d this is as many products as one sweep with an accumulator per map
+// it (16 bits: in two terms), and needs one product with v.  With dv = 2 d this is as many products as one sweep with an accumulator per map
 // (2 d + 2 d + dv against 2 d + 2 dv per pair of tokens) and half the accumulators, and A, not P1 and P2, is rounded: where the maps
 // cancel, rounding them apart would leave an error of the size of what was cancelled.
 // A workgroup has 4 waves: 4 / KW groups of 32 queries, and KW waves that share a tile's keys.
@@ -60,7 +60,7 @@ struct FwdShape {
   static constexpr int MIN_BLOCKS = P == 3 && DP > 32 ? 1 : 2;
 };
 
-template <class T, int DP, int DVP, int KW, bool FINE>
+template <class T, int DP, int DVP, int KW>
 __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void fwd_kernel(Args a) {
   typedef FwdShape<T, DP, DVP> S;
   typedef typename S::KTile KTile;
@@ -231,11 +231,11 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
           p[r] = fmaf(-lam, p2(s2[r], a.c), p1(s1[r], a.c));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const Frag<P> pf = pack8<T>(p + 8 * u), rest = FINE ? rest8<T>(p + 8 * u, pf) : pf;
+          const Frag<P> pf = pack8<T>(p + 8 * u), rest = TWO_TERMS<T> ? rest8<T>(p + 8 * u, pf) : pf;
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
             const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, 32 * i, lane, DVP);
-            if (FINE) accumulate<T>(o[i], vf, rest);
+            if (TWO_TERMS<T>) accumulate<T>(o[i], vf, rest);
             accumulate<T>(o[i], vf, pf);
           }
         }
@@ -357,11 +357,11 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const Frag<P> pf = pack8<T>(p + 8 * u), rest = P == 1 ? rest8<T>(p + 8 * u, pf) : pf;
+      const Frag<P> pf = pack8<T>(p + 8 * u), rest = TWO_TERMS<T> ? rest8<T>(p + 8 * u, pf) : pf;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const Frag<P> vf = VTile::cols(vt, 32 * hh + 16 * u, 32 * j, lane, DVP);
-        if constexpr (P == 1) accumulate<T>(o[j], vf, rest);
+        if (TWO_TERMS<T>) accumulate<T>(o[j], vf, rest);
         accumulate<T>(o[j], vf, pf);
       }
     }
@@ -429,14 +429,14 @@ __global__ __launch_bounds__(THREADS) void split_join(Args a) {
   store4<T>(static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w + c, v[0], v[1], v[2], v[3]);
 }
 
-template <class T, int DP, int DVP, int KW, bool FINE>
+template <class T, int DP, int DVP, int KW>
 int launch_fwd(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
   static LdsAttrOnce once;
-  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW, FINE>), S::LDS)) return -2;
+  if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
   const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
   if (blocks > 0x7fffffffLL) return -3;
-  hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW, FINE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
+  hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
 
@@ -453,9 +453,11 @@ int launch_split(const Args& a, hipStream_t st) {
 }
 
 // Few workgroups (of 128 queries): half as many queries in each, the keys of a tile shared by two waves, so that a workgroup's chain of tiles is
-// shorter.  It pays while the halves leave no CU with more than three; a causal grid, whose longest chain is its time, gains up to two
-// workgroups per CU.  Measured, one wave / two, d = 64, dv = 128, bf16, 4096 tokens: 256 workgroups 192 / 170 us, 384 262 / 271 (d = 32: 199 / 162),
-// 448 265 / 322; causal 256 198 / 140, 480 269 / 261; 512 of 2048 tokens 142 / 132, 768 169 / 183.
+// shorter.  It is more work in all, so fuller grids lose; a causal grid's longest chain is its time, and it gains up to two workgroups per CU.  us, one
+// wave / two, bf16, 2048 tokens, d = 64, dv = 128: 288 workgroups 154 / 156, 384 155 / 156, 480 160 / 187, 576 239 / 238, 768 248 / 281 (256 of 4096
+// tokens 212 / 191; d = 32, dv = 64: 384 117 / 96, 480 118 / 129); causal 384 156 / 111, 480 156 / 140, 576 157 / 166, 768 181 / 193.  The bounds are those
+// of the 16-bit types; in fp32 a causal grid gains beyond them too (1024 workgroups 1134 / 991, d = 32 492 / 406, d = 48 844 / 796; 2048 of d = 48 lose,
+// 1559 / 1591).
 inline bool few_queries(const Args& a) {
   return (long long)a.B * a.H * (((long long)a.N + 127) / 128) <= (a.causal ? 512 : 384);
 }
@@ -463,10 +465,8 @@ inline bool few_queries(const Args& a) {
 template <class T>
 int run_forward(const Args& a, hipStream_t st) {
   const bool few = few_queries(a);
-  constexpr bool HALF = Type<T>::planes == 1;
 #define SCGG_X(DP, DVP) \
-  if (a.d <= DP && a.dv_w <= DVP) \
-    return HALF && a.fine ? launch_fwd<T, DP, DVP, 2, HALF>(a, st) : few ? launch_fwd<T, DP, DVP, 2, false>(a, st) : launch_fwd<T, DP, DVP, 1, false>(a, st);
+  if (a.d <= DP && a.dv_w <= DVP) return few ? launch_fwd<T, DP, DVP, 2>(a, st) : launch_fwd<T, DP, DVP, 1>(a, st);
   SCGG_DIFF_WIDTHS(SCGG_X)
 #undef SCGG_X
   return -1;
