@@ -119,7 +119,7 @@ void plan_dkv(Args& a) {
 // 513 -> 490 us).
 void plan_dq(Args& a) {
   const long long blocks = (long long)a.B * a.H * (((long long)a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
-  long long s = blocks > 0 && blocks <= (tiles < 32 ? 128 : 160) ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;
+  long long s = blocks == 0 ? 1 : blocks <= (tiles < 32 ? 128 : 160) ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;
   if (s > 16) s = 16;
   if (s > tiles / 8) s = tiles / 8;
   a.dq_splits = s < 1 ? 1 : (int)s;

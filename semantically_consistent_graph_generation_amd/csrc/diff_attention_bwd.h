@@ -586,6 +586,7 @@ int launch_dq(const Args& a, hipStream_t st) {
 template <class T, int DP, int DVP>
 int launch_dq_split(const Args& a, hipStream_t st) {
   const long long rows = (long long)a.B * a.H * a.N, quads = rows * 2 * a.d / 4;
+  if (rows == 0) return 0;
   if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
   if (const int rc = launch_dq<T, DP, DVP, 2, 1>(a, st)) return rc;
   hipLaunchKernelGGL(delta_join, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);

@@ -21,3 +21,16 @@ def test_large_problems_round_outputs_only(case, dtype):
     q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, N + M + d + 1)
     mask = mask_of(kind, B, M, g)
     check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal), reference(q, k, v, lam, dout, mask, causal, terms=2))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,N,M", [(0, 1024, 1024), (2, 0, 1024), (0, 5, 9000), (2, 0, 9000), (2, 1024, 0)])
+def test_empty_with_many_keys(B, N, M, causal):
+    """No queries or no keys, at sizes where the plans split: an empty output and gradients of zeros."""
+    from semantically_consistent_graph_generation_amd.attention import diff_attention
+    leaves = [torch.zeros(B, n, h, 32, device="cuda", requires_grad=True) for n, h in ((N, 4), (M, 4), (M, 2))]
+    leaves.append(torch.full((2,), 0.3, device="cuda", requires_grad=True))
+    out = diff_attention(*leaves, causal=causal)
+    assert out.shape == (B, N, 2, 32) and not out.any()
+    for t, gt in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
+        assert gt.shape == t.shape and not gt.any()
