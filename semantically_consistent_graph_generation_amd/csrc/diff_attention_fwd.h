@@ -275,7 +275,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
 // A few rows against many keys: one pass over k and v, the keys split over workgroups.  The rows of a key head's group (queries x
 // heads that share it) are the columns of 32-wide blocks.  A wave takes one map and one half of a tile's keys and keeps its own
 // maximum, sum and P v, which split_join merges.  P is at most 1 here and not yet A, so it is taken in two terms (h + l): the
-// pass waits for memory, the products are free.  Bound: HBM.  16 sequences x 16
+// pass waits for memory, the products are free.  fp16 takes 2^14 P: where one key leads, all others together may matter and each be below its steps.  Bound: HBM.  16 sequences x 16
 // heads on 4, one query each, against 32768 keys, d = 64, dv = 128, bf16: 205 - 209 us for 1.07 GB, 5.1 - 5.2 TB/s (a large copy: 4.9); ragged 169 us for
 // 0.74 GB, 4.4 TB/s.
 template <class T, int DP, int DVP>
@@ -304,6 +304,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
   keys.mask = a.mask ? a.mask + b * a.mb : nullptr;
   keys.words = reinterpret_cast<u64*>(lds + S::WORDS);
   keys.M = a.M;
+  constexpr float UP = __is_same(T, _Float16) ? 16384.f : 1.f;
   const int tiles = (a.M + TILE - 1) / TILE, first = split * a.split_tiles;
   keys.end = first + a.split_tiles < tiles ? first + a.split_tiles : tiles;
 
@@ -347,6 +348,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
     for (int r = 0; r < 16; ++r) {
       p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -tc));
       sum += p[r];
+      p[r] *= UP;
     }
     l = fmaf(l, keep, sum);
     if (__any(keep != 1.f)) {                                    // most tiles leave every maximum as it is
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void s
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int col = 32 * j + 2 * r + 4 * g;
-      if (col < a.dv_w) *reinterpret_cast<f32x4*>(out + map * a.dv_w + col) = f32x4{o[j][r], o[j][r + 1], o[j][r + 2], o[j][r + 3]};
+      if (col < a.dv_w) *reinterpret_cast<f32x4*>(out + map * a.dv_w + col) = f32x4{o[j][r], o[j][r + 1], o[j][r + 2], o[j][r + 3]} * (1.f / UP);
     }
   if (g == 0) { out[2 * a.dv_w + 2 * map] = m; out[2 * a.dv_w + 2 * map + 1] = l; }
 }

@@ -3,7 +3,7 @@ references and tolerances are used here."""
 import pytest
 import torch
 
-from test_gpu_diff_attention import check, make, mask_of, reference, run_all
+from test_gpu_diff_attention import DT, check, make, mask_of, reference, run_all
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,21 @@ def test_empty_with_many_keys(B, N, M, causal):
     assert out.shape == (B, N, 2, 32) and not out.any()
     for t, gt in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
         assert gt.shape == t.shape and not gt.any()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("N,M", [(1, 600), (2, 5000), (40, 300), (1, 40)])
+def test_one_key_leads(N, M, dtype):
+    """One key 17.5 above all others, with a value of zero: the output is the others' share, 2.5e-8 (2^-25.3, less than half of fp16's smallest
+    step) of each value, and it has the accuracy that the entries of A have at any size."""
+    q, k, v, lam, dout, g = make(1, N, M, 1, 1, 32, 64, dtype, N + M, size=1.0)
+    q[:] = q[:, :1]
+    k *= 0.02
+    lead = q[0, 0, 0].double()
+    k[0, M // 3, 0] = (lead * (17.5 * 32 ** 0.5 / float(lead @ lead))).to(k.dtype)
+    v.abs_().mul_(1000.0)
+    v[0, M // 3] = 0
+    lam.zero_()
+    want = reference(q, k, v, lam, dout, None, False, terms=1 if dtype == "fp32" else 2)[:1]
+    assert float(want[0][0].max()) < 1.0 and float((want[0][1] / want[0][0]).max()) < 0.02
+    check(run_all(q, k, v, lam, dout)[:1], want)
