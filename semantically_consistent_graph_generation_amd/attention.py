@@ -13,13 +13,15 @@ read where they lie (a last axis that is not dense, or rows off the 16-byte grid
 and gradients are contiguous and of the inputs' type; statistics, sums and angles are held in 32 bits or more and rounded once.
 Calls enqueue on the current stream of the tensors' device, never synchronise, give equal bits for equal inputs, and can be
 captured into a HIP graph.  A tensor that another stream filled needs that stream's work to be waited for first, as with any
-torch operation.  There is no CPU path (``_lib.ScggError``); second derivatives are not built.
+torch operation.  There is no CPU path (``_lib.ScggError``); second derivatives and forward-mode derivatives are not built, and
+``torch.jit.trace`` is refused.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -44,6 +46,14 @@ def _check_heads(what, name, t, like=None):
             _fail(what, f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")
     elif t.dtype != like.dtype or t.device != like.device:
         _fail(what, f"{name} is {t.dtype} on {t.device}, q is {like.dtype} on {like.device}")
+
+
+def _check_mode(what, *ts):
+    """The launches are seen by reverse-mode autograd and by stream capture, and by nothing else that records torch's operations."""
+    if torch.jit.is_tracing():
+        _fail(what, "it cannot be traced (the trace would hold the empty outputs and not the kernels)")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        _fail(what, "forward-mode derivatives are not built")
 
 
 def _check_device(what, t):
@@ -207,6 +217,7 @@ def _rope(what, q, k, wq, wk, positions, sections, theta, interleaved, eps):
             _fail(what, f"{name} has to be [{D}], float32 or {q.dtype}, on {q.device}")
     if wq is not None and wk is not None and wq.dtype != wk.dtype:
         _fail(what, f"q_weight is {wq.dtype}, k_weight is {wk.dtype}: one type is needed")
+    _check_mode(what, q, k, wq, wk, positions)
     _check_device(what, q)
     q, k = _dense_rows(q), None if k is None else _dense_rows(k)
     wq, wk = (None if w is None else w.contiguous() for w in (wq, wk))
@@ -341,6 +352,7 @@ def diff_attention(q, k, v, lam, key_mask=None, causal=False, scale=None):
             _fail(what, f"key_mask {tuple(key_mask.shape)} on {key_mask.device}: [{B}, {M}] on {q.device} is needed")
         if M > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
+    _check_mode(what, q, k, v, lam)
     _check_device(what, q)
     q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
     cfg = (bool(causal), scale)

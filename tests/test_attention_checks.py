@@ -180,3 +180,28 @@ def test_diff_c_entry_refuses_outputs_off_the_grid_and_scales_out_of_range():
         assert L.scgg_diff_attention_backward(C.byref(diff_args(**{n: 4104})), 4096, 1 << 30, None) != 0 and "aligned" in L.scgg_last_error().decode()
     a = diff_args(scale=3e38)
     assert L.scgg_diff_attention_forward(C.byref(a), None, 0, None) != 0 and "scale" in L.scgg_last_error().decode()
+
+
+def calls():
+    """(operator of its tensors, the tensors) of every entry point."""
+    q, k, v = Z(1, 3, 2, 8), Z(1, 3, 2, 8), Z(1, 3, 1, 8)
+    return [(lambda q, k, pos: A.axial_rope(q, k, pos, (4,))[0], (q, k, Z(1, 3, 1))),
+            (lambda q, k, wq, wk, pos: A.qk_norm_rope(q, k, wq, wk, pos, (4,))[0], (q, k, Z(8), Z(8), Z(1, 3, 1))),
+            (lambda q, k, v, lam: A.diff_attention(q, k, v, lam), (q, k, v, Z(1)))]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_and_traces_are_refused(which, monkeypatch):
+    """A tangent would be dropped, and a trace would return memory that nothing wrote: both go past the operators' autograd function."""
+    from torch.autograd import forward_ad as fw
+    monkeypatch.setattr(A, "_check_device", lambda *a: None)
+    monkeypatch.setattr(A, "_call", lambda *a: 0)
+    f, ts = calls()[which]
+    f(*ts)
+    for i in range(len(ts)):
+        with fw.dual_level():
+            f(*ts)                                                    # no tangents: an ordinary call
+            with pytest.raises(_lib.ScggError, match="forward-mode"):
+                f(*ts[:i], fw.make_dual(ts[i], torch.ones_like(ts[i])), *ts[i + 1:])
+    with pytest.raises(_lib.ScggError, match="traced"):
+        torch.jit.trace(f, ts)
