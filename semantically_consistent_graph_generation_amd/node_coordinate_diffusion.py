@@ -203,7 +203,7 @@ class SiT(nn.Module):
             x = (x - (1.0 - al) / math.sqrt(1.0 - ah) * eps) / math.sqrt(al)
             if i > 1:
                 if noise is None and z.numel():
-                    _lib.check(_lib.lib().scgg_philox_normal_rows(_lib.ptr(z), B, n, seed, graph_id_base, i, _lib.stream_ptr()), "philox_normal_rows")
+                    _lib.check(attn_ops._call(x.device, _lib.lib().scgg_philox_normal_rows, _lib.ptr(z), B, n, seed, graph_id_base, i), "philox_normal_rows")
                 x = x + math.sqrt(be) * (z if noise is None else noise[k].float())
         return x.masked_fill(~mask[..., None], 0.0)
 

@@ -205,3 +205,23 @@ def test_forward_mode_and_traces_are_refused(which, monkeypatch):
                 f(*ts[:i], fw.make_dual(ts[i], torch.ones_like(ts[i])), *ts[i + 1:])
     with pytest.raises(_lib.ScggError, match="traced"):
         torch.jit.trace(f, ts)
+
+
+def test_differential_sampler_draws_on_its_tensors_device(monkeypatch):
+    """The draws run on the stream and with the device of the tensors, which need not be the current ones."""
+    from semantically_consistent_graph_generation_amd import node_coordinate_diffusion as N
+    model = N.SiT(attention="differential", num_transformer_blocks=1, noise_steps=4)
+    seen = []
+
+    class Lib:
+        @staticmethod
+        def scgg_philox_normal_rows(*a):
+            raise AssertionError("not on the tensors' device")
+    monkeypatch.setattr(N._lib, "lib", lambda: Lib)
+    monkeypatch.setattr(N._lib, "ptr", lambda t: t)
+    monkeypatch.setattr(N._lib, "stream_ptr", lambda: None)
+    monkeypatch.setattr(A, "_call", lambda device, fn, *a: seen.append((device, fn, a)) or 0)
+    monkeypatch.setattr(model, "_forward_differential", lambda x, t, m: torch.zeros_like(x))
+    x = Z(2, 3, 3)
+    model.sample(x, torch.ones(2, 3, dtype=torch.bool), seed=5, graph_id_base=7)
+    assert [(d, f is Lib.scgg_philox_normal_rows, a[1:]) for d, f, a in seen] == [(x.device, True, (2, 3, 5, 7, i)) for i in (3, 2)]
