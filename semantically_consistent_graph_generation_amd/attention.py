@@ -321,7 +321,9 @@ def diff_attention(q, k, v, lam, key_mask=None, causal=False, scale=None):
     (query heads h share the key head ``h // (H / Hkv)``).  d and dv: multiples of 8, d <= 64, dv <= 128.  ``lam``: [H] or a
     scalar, a float32 tensor (differentiable) or a number.  ``key_mask`` [B,M], bool or uint8: True keys are seen; what hidden
     keys and their values hold does not matter.  ``causal``: query i sees the keys j <= i + M - N (the last query sees all of
-    them).  ``scale`` > 0, default d ** -0.5.  A query that sees no key gives zeros, and no gradient.  Returns [B,N,H,dv].
+    them); a key that ``causal`` hides from some queries only has to be finite, as its value is multiplied by their zeros.  ``scale`` > 0,
+    default d ** -0.5.  A query that sees no key gives zeros, and no gradient, whatever it and its upstream gradient hold.  float32
+    entries are split into terms: an infinity that is seen gives NaN.  Returns [B,N,H,dv].
 
     One or a few queries against many keys (a new token against a cache) split the keys over the GPU.  With N = M short or long
     the maps are never stored."""

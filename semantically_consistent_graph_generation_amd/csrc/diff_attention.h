@@ -339,6 +339,7 @@ struct Prob {
     const float e = __builtin_amdgcn_exp2f(fmaf(s, c, -m));
     return folded ? e : e * f;
   }
+  __device__ __forceinline__ bool never() const { return folded ? m == INFINITY : f == 0.f; }   // the query sees no key
 };
 
 // ------------------------------------------------------------------------------------------------ staging

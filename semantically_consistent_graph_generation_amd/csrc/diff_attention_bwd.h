@@ -62,7 +62,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
     mc[i] = st.x;
     il[i] = st.y;
   }
-  load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on, a.dv_w, g);
+  const bool seeing = il[0] != 0.f || il[1] != 0.f;   // a query that sees no key gets and gives no gradient, whatever its dO holds
+  load_rows<T, DVP>(gf, static_cast<const T*>(a.dout) + b * a.gb + (long long)q * a.gn + (long long)h * a.gh, q_on && seeing, a.dv_w, g);
   // Odd queries take - dO: the matrix instructions round dP with a bias of one sign (fp16: 1e-2 of a step), and dlambda, the sum of P dP over all
   // queries, would add it up (2e-5 of 30 over 1554 queries); so it has the other sign in every second one.
   const float side = (l31 & 1) ? -1.f : 1.f;
@@ -173,6 +174,7 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
       delta[1] = box[(w0 * 3 + 1) * 32 + l31] + box[(w0 * 3 + 4) * 32 + l31];
       top = fmaxf(box[(w0 * 3 + 2) * 32 + l31], box[(w0 * 3 + 5) * 32 + l31]);
     }
+    if (il[0] == 0.f && il[1] == 0.f) delta[0] = delta[1] = top = 0.f;
     if (q_on && kw == 0 && g == 0) {
       float* dst = (PHASE == 1 ? a.part + (long long)split * a.B * a.H * 3 * a.N : a.delta) + (long long)bh * 3 * a.N + q;
       dst[0] = delta[0];
@@ -260,7 +262,8 @@ __global__ __launch_bounds__(THREADS, (DqShape<T, DP, DVP>::MIN_BLOCKS)) void dq
       for (int r = 0; r < 16; r += 4) {
         const int col = 32 * j + 2 * r + 4 * g;
         if (col >= a.d) continue;
-        const f32x4 v = {o[i][j][r] * f, o[i][j][r + 1] * f, o[i][j][r + 2] * f, o[i][j][r + 3] * f};
+        f32x4 v = {o[i][j][r] * f, o[i][j][r + 1] * f, o[i][j][r + 2] * f, o[i][j][r + 3] * f};
+        if (prob[0].never() && prob[1].never()) v = f32x4{0.f, 0.f, 0.f, 0.f};
         if constexpr (PHASE == 2) *reinterpret_cast<f32x4*>(part + col) = v;
         else store4<T>(dst + col, v[0], v[1], v[2], v[3]);
       }
@@ -395,8 +398,13 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
     const long long q_first = (long long)kt * BK - off;
     if (q_first > 0) t_first = q_first / TQ < n_tiles ? (int)(q_first / TQ) : n_tiles;
   }
-  // a workgroup whose keys are all hidden has nothing to sum
-  const bool any = __syncthreads_or(k_on);
+  // the first of the workgroup's keys that the mask leaves; a workgroup that has none has nothing to sum
+  int* firsts = reinterpret_cast<int*>(rowst + 4);
+  const u64 on_keys = __ballot(k_on);
+  if (lane == 0) firsts[wave] = on_keys != 0 ? kt * BK + 32 * wave + __builtin_ctzll(on_keys) : a.M;
+  __syncthreads();
+  const int first_key = min(min(firsts[0], firsts[1]), min(firsts[2], firsts[3]));
+  const bool any = first_key < a.M;
   Stage<T, 2 * DP, 2, TQ> qs;
   Stage<T, DVP, 1, TQ> gs;
   qs.init(a.qn, a.qh, a.d, tid);
@@ -406,12 +414,14 @@ __global__ __launch_bounds__(THREADS, (DkvShape<T, DP, DVP>::MIN_BLOCKS)) void d
   auto load = [&](int hg, int t) {
     const int h = hk * group + hg;
     const long long left = (long long)a.N - (long long)t * TQ;
-    const u64 bits = left >= TQ ? ~0ull : (1ull << left) - 1;
+    u64 bits = left >= TQ ? ~0ull : (1ull << left) - 1;
+    const long long from = a.causal ? first_key - off - (long long)t * TQ : 0;   // queries before it see none of the keys (and may see none at all):
+    if (from > 0) bits &= from < 64 ? ~0ull << from : 0ull;                      // whatever they and their dO hold, they are zeros here
     const long long bh = (long long)b * a.H + h;
     const int n = t * TQ + lane % TQ;                                  // waves 0, 1: statistics of map 0, 1; wave 2: both deltas
     rlam = a.lambda[h];
     rs = wave < 2 ? make_float2(INFINITY, 0.f) : make_float2(0.f, 0.f);
-    if (n < a.N) {
+    if (n < a.N && lane % TQ >= from) {
       if (wave < 2) rs = a.stats[(bh * 2 + wave) * a.N + n];
       else if (wave == 2) rs = make_float2(a.delta[bh * 3 * a.N + n], a.delta[(bh * 3 + 1) * a.N + n]);
     }

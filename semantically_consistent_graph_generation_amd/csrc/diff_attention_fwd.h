@@ -76,7 +76,7 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
   const int bh = id / q_tiles, qt = a.causal ? q_tiles - 1 - (int)(id - bh * q_tiles) : (int)(id - bh * q_tiles);   // causal: long ones first
   const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
   const int q = qt * BQ + 32 * qw + l31;
-  const bool q_on = q < a.N;
+  bool q_on = q < a.N;                                         // the lane's query is to be written
   const long long off = (long long)a.M - a.N;                  // causal: query q sees the keys <= q + off
   const T* kp = static_cast<const T*>(a.k) + b * a.kb + 2ll * hk * a.kh;
   const T* vp = static_cast<const T*>(a.v) + b * a.vb + (long long)hk * a.vh;
@@ -189,6 +189,11 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
     il[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
     if (a.stats != nullptr && q_on && kw == 0 && g == 0)
       a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + q] = make_float2(mc[i], il[i]);
+  }
+  if (q_on && il[0] == 0.f && il[1] == 0.f) {                  // sees nothing: zeros, whatever the tiles hold for others
+    if (kw == 0 && g == 0)
+      for (int col = 0; col < a.dv_w; col += 4) store4<T>(static_cast<T*>(a.out) + (((long long)b * a.N + q) * a.H + h) * a.dv_w + col, 0.f, 0.f, 0.f, 0.f);
+    q_on = false;
   }
   const float lam = a.lambda[h];
   float up = 1.f;
@@ -405,6 +410,7 @@ __global__ __launch_bounds__(THREADS) void split_join(Args a) {
     w[i] = l == 0.f ? 0.f : 1.f / l;
     if (a.stats != nullptr && threadIdx.x == 0) a.stats[((long long)(b * a.H + h) * 2 + i) * a.N + n] = make_float2(mc[i], w[i]);
   }
+  const bool none = w[0] == 0.f && w[1] == 0.f;                    // sees nothing: zeros, whatever the parts hold
   w[1] *= -a.lambda[h];
   const int c = 4 * (lane & 31), side = lane >> 5;                 // lanes 0..31: P1 v, 32..63: P2 v; four columns each
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -428,6 +434,7 @@ __global__ __launch_bounds__(THREADS) void split_join(Args a) {
   __syncthreads();
   if (threadIdx.x >= 32 || c >= a.dv_w) return;
   v = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+  if (none) v = f32x4{0.f, 0.f, 0.f, 0.f};
   store4<T>(static_cast<T*>(a.out) + (((long long)b * a.N + n) * a.H + h) * a.dv_w + c, v[0], v[1], v[2], v[3]);
 }
 

@@ -52,3 +52,37 @@ def test_one_key_leads(N, M, dtype):
     want = reference(q, k, v, lam, dout, None, False, terms=1 if dtype == "fp32" else 2)[:1]
     assert float(want[0][0].max()) < 1.0 and float((want[0][1] / want[0][0]).max()) < 0.02
     check(run_all(q, k, v, lam, dout)[:1], want)
+
+
+def empty_rows(B, N, M, mask):
+    """[B,N]: causal queries that see no key."""
+    first = torch.where(mask.any(1), mask.int().argmax(1), torch.full((B,), M, device="cuda"))
+    return torch.arange(N, device="cuda")[None] + (M - N) < first[:, None]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("case", [(2, 300, 300, 2, 1, 64, 128), (2, 500, 400, 2, 2, 32, 64), (3, 70, 64, 4, 2, 48, 96), (2, 90, 1300, 1, 1, 64, 64),
+                                  (2, 700, 2200, 2, 1, 64, 128), (2, 9, 600, 2, 1, 32, 32), (8, 200, 200, 64, 32, 64, 128)], ids=str)
+def test_rows_that_see_nothing_may_hold_anything(case, dtype):
+    """Causal sequences padded on the left (and N > M): what q and dO hold in the rows that see no key reaches no output and no gradient."""
+    B, N, M, H, Hkv, d, dv = case
+    q, k, v, lam, dout, g = make(B, N, M, H, Hkv, d, dv, dtype, N + M + 5)
+    start = torch.randint(M // 2, M, (B,), generator=g, device="cuda")
+    start[0] = max(2 * M // 3, M - N + 40 if M > N + 40 else 0)
+    mask = torch.arange(M, device="cuda")[None] >= start[:, None]
+    empty = empty_rows(B, N, M, mask)
+    assert empty.any() and not empty.all()
+    clean = run_all(q, k, v, lam, dout, key_mask=mask, causal=True)
+    q2, dout2 = q.clone(), dout.clone()
+    for i, x in enumerate((float("nan"), float("inf"), float("-inf"), torch.finfo(DT[dtype]).max)):
+        spot = empty & (torch.arange(N, device="cuda") % 4 == i)
+        q2[spot], dout2[spot] = x, x
+    for name, a, b in zip(("out", "dq", "dk", "dv", "dlam"), clean, run_all(q2, k, v, lam, dout2, key_mask=mask, causal=True)):
+        assert torch.isfinite(a).all() and torch.equal(a, b), name
+    assert not clean[0][empty].any() and not clean[1][empty].any()
+    # a value that other rows see and that is not finite does not change what such a row gives
+    v2 = v.clone()
+    v2[:, -1] = float("nan")
+    lam2 = torch.full_like(lam, float("inf"))
+    for got in (run_all(q, k, v2, lam, dout, key_mask=mask, causal=True), run_all(q, k, v, lam2, dout, key_mask=mask, causal=True)):
+        assert not got[0][empty].any() and not got[1][empty].any()
