@@ -183,6 +183,17 @@ __global__ __launch_bounds__(THREADS, (FwdShape<T, DP, DVP>::MIN_BLOCKS)) void f
       l[i] = l0;
     }
   }
+  // a base far below the maximum (the sum is then that large) moves up to it: the backward multiplies 2^(c s - m) by dP before it takes 1 / sum, and
+  // |dP| of 2^48 and more would overflow with the 2^80 that the sweep allows
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (l[i] > 0x1p32f) {
+      int e;
+      l[i] = frexpf(l[i], &e);
+      const float t = m[i] + (float)e;
+      l[i] *= __builtin_amdgcn_exp2f((m[i] - t) + (float)e);   // what the rounding of t left
+      m[i] = t;
+    }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {   // a query that sees nothing: every 2^(c s - mc) is 0
     mc[i] = l[i] == 0.f ? INFINITY : m[i];

@@ -86,3 +86,20 @@ def test_rows_that_see_nothing_may_hold_anything(case, dtype):
     lam2 = torch.full_like(lam, float("inf"))
     for got in (run_all(q, k, v2, lam, dout, key_mask=mask, causal=True), run_all(q, k, v, lam2, dout, key_mask=mask, causal=True)):
         assert not got[0][empty].any() and not got[1][empty].any()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("N,M,causal", [(40, 130, False), (150, 300, True), (20, 2000, False)])
+def test_large_gradients_and_a_late_maximum(N, M, causal, dtype):
+    """dP of 2^74 and, behind a first tile of scores near 0, keys whose scores are 45 (2^65 in the exponents) and 50 (2^72) larger."""
+    q, k, v, lam, dout, g = make(1, N, M, 1, 1, 32, 64, dtype, N + M + 1, size=1.0)
+    q[:] = q[:, :1]
+    k *= 0.02
+    for at, score in ((70, 45.0), (75, 45.0), (128, 50.0)):
+        for i in range(2):
+            lead = q[0, 0, i].double()
+            k[0, at, i] = (lead * (score * 32 ** 0.5 / float(lead @ lead))).to(k.dtype)
+    v, dout = v * 2.0 ** 35, dout * 2.0 ** 35
+    want = reference(q, k, v, lam, dout, None, causal, terms=1 if dtype == "fp32" else 2)
+    assert float(want[1][0].abs().max()) > 2.0 ** 48
+    check(run_all(q, k, v, lam, dout, causal=causal), want)
