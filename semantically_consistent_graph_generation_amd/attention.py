@@ -41,7 +41,7 @@ def _check_heads(what, name, t, like=None):
         _fail(what, f"{name} has to be a tensor")
     if t.dim() != 4:
         _fail(what, f"{name} has to be [B, tokens, heads, width], got {tuple(t.shape)}")
-    if like is None:
+    if like is None or like is t:
         if t.dtype not in _DTYPES:
             _fail(what, f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")
     elif t.dtype != like.dtype or t.device != like.device:

@@ -225,3 +225,9 @@ def test_differential_sampler_draws_on_its_tensors_device(monkeypatch):
     x = Z(2, 3, 3)
     model.sample(x, torch.ones(2, 3, dtype=torch.bool), seed=5, graph_id_base=7)
     assert [(d, f is Lib.scgg_philox_normal_rows, a[1:]) for d, f, a in seen] == [(x.device, True, (2, 3, 5, 7, i)) for i in (3, 2)]
+
+
+def test_diff_attention_refuses_types_that_all_tensors_share():
+    q, k, v = Z(2, 5, 4, 32), Z(2, 7, 4, 32), Z(2, 7, 2, 64)
+    for t in (torch.float64, torch.int32, torch.float8_e4m3fn):
+        refused(A.diff_attention, q.to(t), k.to(t), v.to(t), Z(2), match="are supported")
