@@ -233,7 +233,8 @@ def axial_rope(q, k, positions, sections, theta=10000.0, interleaved=False):
     turn with axis a, the j-th of them by the angle ``positions[.., a] * theta ** (-j / sections[a])``; pairs behind the last
     section are left as they are.  A pair is (x[2i], x[2i+1]) if ``interleaved``, else (x[i], x[i + D/2]).  Angles are formed
     in 64 bits, so far positions keep theirs.  Returns (q', k'), contiguous; differentiable in q and k."""
-    if len(tuple(sections)) == 0:
+    sections = tuple(sections)
+    if not sections:
         _fail("axial_rope", "sections name no axis")
     return _rope("axial_rope", q, k, None, None, positions, sections, theta, interleaved, 0.0)
 

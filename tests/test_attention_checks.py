@@ -231,3 +231,11 @@ def test_diff_attention_refuses_types_that_all_tensors_share():
     q, k, v = Z(2, 5, 4, 32), Z(2, 7, 4, 32), Z(2, 7, 2, 64)
     for t in (torch.float64, torch.int32, torch.float8_e4m3fn):
         refused(A.diff_attention, q.to(t), k.to(t), v.to(t), Z(2), match="are supported")
+
+
+def test_sections_from_an_iterator():
+    """Counted once: an iterator that the check used up would leave no axis, and no rotation."""
+    q, pos = Z(2, 5, 4, 32), Z(2, 5, 3)
+    refused(A.axial_rope, q, None, pos, iter((6, 6, 5)), match="16 pairs")
+    refused(A.axial_rope, q, None, pos, (n for n in (6, 5, 5)), match="GPU")
+    refused(A.axial_rope, q, None, pos[..., :2], map(int, "655"), match="is needed")
