@@ -41,6 +41,8 @@ def _check_heads(what, name, t, like=None):
         _fail(what, f"{name} has to be a tensor")
     if t.dim() != 4:
         _fail(what, f"{name} has to be [B, tokens, heads, width], got {tuple(t.shape)}")
+    if max(t.shape) > 2 ** 31 - 1:                             # the C side's extents are 32 bits and would take what is left of it
+        _fail(what, f"{name} {tuple(t.shape)}: too many entries along an axis")
     if like is None or like is t:
         if t.dtype not in _DTYPES:
             _fail(what, f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")

@@ -239,3 +239,16 @@ def test_sections_from_an_iterator():
     refused(A.axial_rope, q, None, pos, iter((6, 6, 5)), match="16 pairs")
     refused(A.axial_rope, q, None, pos, (n for n in (6, 5, 5)), match="GPU")
     refused(A.axial_rope, q, None, pos[..., :2], map(int, "655"), match="is needed")
+
+
+def test_extents_past_32_bits_are_refused(monkeypatch):
+    """2^32 + 5 tokens would be taken as 5: the rest of the output would keep what its memory held."""
+    monkeypatch.setattr(A, "_check_device", lambda *a: None)
+    monkeypatch.setattr(A, "_call", lambda *a: pytest.fail("launched"))
+    far = 2 ** 32 + 5
+    q = Z(1, 1, 2, 8)
+    refused(A.axial_rope, q.expand(1, far, 2, 8), None, Z(1, 1).expand(far, 1), (4,), match="too many")
+    refused(A.axial_rope, q, Z(1, 1, 1, 8).expand(1, 1, far, 8), Z(1, 1), (4,), match="too many")
+    refused(A.qk_norm_rope, q.expand(far, 1, 2, 8), None, Z(8), None, match="too many")
+    refused(A.diff_attention, q, q.expand(1, far, 2, 8), Z(1, 1, 1, 8).expand(1, far, 1, 8), 0.5, match="too many")
+    refused(A.diff_attention, q.expand(1, far, 2, 8), q, Z(1, 1, 1, 8), 0.5, match="too many")
