@@ -27,6 +27,7 @@ namespace {
 
 constexpr int ROPE_MAX_PAIRS = 128;      // head width up to 256
 constexpr int ROPE_TILE = 64;            // tokens per workgroup tile at most
+constexpr int ROPE_GROUPS = 1 << 23;     // workgroups at most (a launch counts its threads in 32 bits); each takes every gridDim.x-th tile
 constexpr int ROPE_TRAIN_GROUPS = 2048;  // workgroups of a backward with weights, q's and k's: rows of the partial sums
 
 struct RopeSide {
@@ -360,7 +361,7 @@ void rope_plan(const scgg_rope_args* p, bool bwd, bool norm, RopePlan* out) {
     auto idle = [&](long long t) { return (double)((t * own + groups - 1) / groups * groups) / (double)(t * own); };
     for (long long t = tile, least = tile / 2 + 1; t >= least; --t)         // of the sizes down to half: the one whose last round is fullest
       if (idle(t) < idle(tile) - 1e-9) tile = t;
-    const long long tiles = (tokens + tile - 1) / tile, cap = apart ? ROPE_TRAIN_GROUPS * own / all : tiles;
+    const long long tiles = (tokens + tile - 1) / tile, cap = apart ? ROPE_TRAIN_GROUPS * own / all : ROPE_GROUPS;
     out->tile[s] = (int)tile;
     out->blocks[s] = tiles < cap ? tiles : cap < 1 ? 1 : cap;
     const size_t lds = p->n_sections > 0 ? (size_t)tile * half * sizeof(float2) : 0;
@@ -412,7 +413,6 @@ int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspac
   rope_plan(p, bwd, norm, &plan);
   RopeArgs a = {};
   const long long blocks = plan.blocks[0] + plan.blocks[1];
-  if (blocks > 0x7fffffffLL) return fail("%s: too many tokens for one launch", what);
   for (int s = 0; s < 2; ++s) {
     RopeSide& q = a.side[s];
     q.x = p->x[s]; q.g = p->g[s]; q.y = p->y[s]; q.w = p->weight[s]; q.heads = p->heads[s];

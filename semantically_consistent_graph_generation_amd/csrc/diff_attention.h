@@ -34,6 +34,7 @@ typedef unsigned long long u64;
 
 constexpr int TILE = 64;          // keys (or queries) per tile: one bit each in a wave-wide ballot
 constexpr int THREADS = 256;
+constexpr long long MAX_BLOCKS = 0xffffffffll / THREADS;   // a launch counts its threads in 32 bits
 
 struct Args {
   const void *q, *k, *v, *dout;

@@ -585,10 +585,10 @@ __global__ __launch_bounds__(256) void dkv_join(Args a, long long quads) {
 template <class T, int DP, int DVP, int KW, int PHASE>
 int launch_dq(const Args& a, hipStream_t st) {
   typedef DqShape<T, DP, DVP> S;
+  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW)) * (PHASE == 0 ? 1 : a.dq_splits);
+  if (blocks > MAX_BLOCKS) return -3;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dq_kernel<T, DP, DVP, KW, PHASE>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW)) * (PHASE == 0 ? 1 : a.dq_splits);
-  if (blocks > 0x7fffffffLL) return -3;
   if (blocks > 0) hipLaunchKernelGGL((dq_kernel<T, DP, DVP, KW, PHASE>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
@@ -597,7 +597,7 @@ template <class T, int DP, int DVP>
 int launch_dq_split(const Args& a, hipStream_t st) {
   const long long rows = (long long)a.B * a.H * a.N, quads = rows * 2 * a.d / 4;
   if (rows == 0) return 0;
-  if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
+  if ((quads + 255) / 256 > MAX_BLOCKS) return -3;
   if (const int rc = launch_dq<T, DP, DVP, 2, 1>(a, st)) return rc;
   hipLaunchKernelGGL(delta_join, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, a, rows);
   if (const int rc = launch_dq<T, DP, DVP, 2, 2>(a, st)) return rc;
@@ -608,10 +608,10 @@ int launch_dq_split(const Args& a, hipStream_t st) {
 template <class T, int DP, int DVP, int WHAT>
 int launch_dkv(const Args& a, hipStream_t st) {
   typedef DkvShape<T, DP, DVP> S;
+  const long long blocks = (long long)a.B * a.Hkv * ((a.M + BK - 1) / BK) * a.splits;
+  if (blocks > MAX_BLOCKS) return -3;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&dkv_kernel<T, DP, DVP, WHAT>), S::lds(WHAT))) return -2;
-  const long long blocks = (long long)a.B * a.Hkv * ((a.M + BK - 1) / BK) * a.splits;
-  if (blocks > 0x7fffffffLL) return -3;
   if (blocks > 0) hipLaunchKernelGGL((dkv_kernel<T, DP, DVP, WHAT>), dim3((unsigned)blocks), dim3(THREADS), S::lds(WHAT), st, a);
   return 0;
 }
@@ -634,7 +634,7 @@ int launch_bwd(const Args& a, hipStream_t st) {
   }
   const long long quads = (long long)a.B * a.M * a.Hkv * (2 * a.d + a.dv_w) / 4;
   if (a.splits > 1 && quads > 0) {
-    if ((quads + 255) / 256 > 0x7fffffffLL) return -3;
+    if ((quads + 255) / 256 > MAX_BLOCKS) return -3;
     hipLaunchKernelGGL((dkv_join<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, quads);
   }
   return 0;

@@ -452,10 +452,10 @@ __global__ __launch_bounds__(THREADS) void split_join(Args a) {
 template <class T, int DP, int DVP, int KW>
 int launch_fwd(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
+  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
+  if (blocks > MAX_BLOCKS) return -3;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&fwd_kernel<T, DP, DVP, KW>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.H * ((a.N + 128 / KW - 1) / (128 / KW));
-  if (blocks > 0x7fffffffLL) return -3;
   hipLaunchKernelGGL((fwd_kernel<T, DP, DVP, KW>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   return 0;
 }
@@ -463,10 +463,10 @@ int launch_fwd(const Args& a, hipStream_t st) {
 template <class T, int DP, int DVP>
 int launch_split(const Args& a, hipStream_t st) {
   typedef FwdShape<T, DP, DVP> S;
+  const long long blocks = (long long)a.B * a.Hkv * (((long long)a.N * (a.H / a.Hkv) + 31) / 32) * a.splits;
+  if (blocks > MAX_BLOCKS || (long long)a.B * a.N * a.H > MAX_BLOCKS) return -3;
   static LdsAttrOnce once;
   if (set_max_dynamic_lds(once, reinterpret_cast<const void*>(&split_kernel<T, DP, DVP>), S::LDS)) return -2;
-  const long long blocks = (long long)a.B * a.Hkv * (((long long)a.N * (a.H / a.Hkv) + 31) / 32) * a.splits;
-  if (blocks > 0x7fffffffLL || (long long)a.B * a.N * a.H > 0x7fffffffLL) return -3;
   hipLaunchKernelGGL((split_kernel<T, DP, DVP>), dim3((unsigned)blocks), dim3(THREADS), S::LDS, st, a);
   hipLaunchKernelGGL((split_join<T>), dim3((unsigned)(a.B * a.N * a.H)), dim3(THREADS), 0, st, a);
   return 0;

@@ -252,3 +252,16 @@ def test_extents_past_32_bits_are_refused(monkeypatch):
     refused(A.qk_norm_rope, q.expand(far, 1, 2, 8), None, Z(8), None, match="too many")
     refused(A.diff_attention, q, q.expand(1, far, 2, 8), Z(1, 1, 1, 8).expand(1, far, 1, 8), 0.5, match="too many")
     refused(A.diff_attention, q.expand(1, far, 2, 8), q, Z(1, 1, 1, 8), 0.5, match="too many")
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are made up")
+def test_diff_c_entry_refuses_grids_past_the_launch_limit():
+    """Workgroups of 256 threads, 2^32 threads and more: refused before anything is set up or launched."""
+    L = _lib.lib()
+    lots = dict(B=2 ** 24, N=1, H=1, Hkv=1, d=8, dv=8)
+    for kw in (dict(lots, M=4), dict(lots, M=600), dict(lots, B=2 ** 19, N=32, M=600)):
+        a = diff_args(**kw)
+        need = L.scgg_diff_attention_forward_workspace_bytes(C.byref(a))
+        assert L.scgg_diff_attention_forward(C.byref(a), 4096, need, None) != 0 and "one launch" in L.scgg_last_error().decode()
+    a = diff_args(**lots, M=4)
+    assert L.scgg_diff_attention_backward(C.byref(a), 4096, 1 << 62, None) != 0 and "one launch" in L.scgg_last_error().decode()

@@ -103,3 +103,15 @@ def test_large_gradients_and_a_late_maximum(N, M, causal, dtype):
     want = reference(q, k, v, lam, dout, None, causal, terms=1 if dtype == "fp32" else 2)
     assert float(want[1][0].abs().max()) > 2.0 ** 48
     check(run_all(q, k, v, lam, dout, causal=causal), want)
+
+
+def test_rope_over_more_tiles_than_a_launch_has_workgroups():
+    """2^30 + 77 tokens of one pair (2^24 + 2 tiles of 64 tokens), all at the same position."""
+    from semantically_consistent_graph_generation_amd.attention import axial_rope
+    N = 2 ** 30 + 77
+    q = torch.empty(1, N, 1, 2, dtype=torch.bfloat16, device="cuda")
+    q[..., 0], q[..., 1] = 1.0, 0.5
+    pos = torch.tensor([[0.7]], device="cuda")
+    want, _ = axial_rope(q[:, :64], None, pos.expand(64, 1), (1,))
+    got, _ = axial_rope(q, None, pos.expand(N, 1), (1,))
+    assert bool((got.view(torch.int32) == want.view(torch.int32)[0, 0, 0, 0]).all())
