@@ -234,7 +234,7 @@ def axial_rope(q, k, positions, sections, theta=10000.0, interleaved=False):
     real (coordinates) or whole (voxel or token indices), float32 / float64 / int32 / int64.  ``sections[a]`` pairs of a head
     turn with axis a, the j-th of them by the angle ``positions[.., a] * theta ** (-j / sections[a])``; pairs behind the last
     section are left as they are.  A pair is (x[2i], x[2i+1]) if ``interleaved``, else (x[i], x[i + D/2]).  Angles are formed
-    in 64 bits, so far positions keep theirs.  Returns (q', k'), contiguous; differentiable in q and k."""
+    in two terms of 64 bits, so positions as far as 64 bits hold them keep theirs.  Returns (q', k'), contiguous; differentiable in q and k."""
     sections = tuple(sections)
     if not sections:
         _fail("axial_rope", "sections name no axis")

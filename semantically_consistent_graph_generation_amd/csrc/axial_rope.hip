@@ -7,8 +7,8 @@
 //   u = R^T g,  dw = sum over tokens and heads of u h,  dx = (u w - h mean(u w h)) / sqrt(mean x^2 + eps).
 //
 // Bound: HBM (x in, y out; backward g, x in, dx out).  A workgroup takes a tile of tokens.  Its threads first form the cosines
-// and sines of the tile, each once for all heads of q and k: positions reach 1e6 and beyond, so the angle is a product in
-// 64 bits, reduced to an eighth of a turn there, and only then rounded to 32.  Then the heads stream through, 16 B per load: a
+// and sines of the tile, each once for all heads of q and k: positions reach 1e6 and beyond, so the angle is a product in two
+// 64-bit terms, reduced to an eighth of a turn there, and only then rounded to 32.  Then the heads stream through, 16 B per load: a
 // head belongs to a power of two of lanes that hold whole pairs, so the rotation needs no exchange and the norm one butterfly.
 // In the backward of a norm a workgroup belongs to q or to k, so that a lane has one side's weights and sums (281 -> 258 us for 4 x 16384 tokens of
 // 20 bf16 heads of 128; 252 now, the forward 162, together 1.68 GB at 4.0 TB/s); elsewhere it takes both, and the cosines are formed once (21
@@ -48,7 +48,8 @@ struct RopeArgs {
   int flat;                    // every batch stride is N token strides: the token's number is its place
   unsigned tokens;
   float eps;
-  double turn[ROPE_MAX_PAIRS]; // theta^(-j / n_a) / (2 pi)
+  double turn[ROPE_MAX_PAIRS]; // theta^(-j / n_a) / (2 pi), and what its rounding left
+  double turn_low[ROPE_MAX_PAIRS];
   uint8_t axis[ROPE_MAX_PAIRS];
 };
 
@@ -73,13 +74,17 @@ __device__ __forceinline__ double rope_position(const RopeArgs& a, unsigned tok,
   return (double)static_cast<const int64_t*>(a.pos)[at];
 }
 
-// cos and sin of `turns` whole turns.  The nearest quarter turn comes off in 64 bits (adding 1.5 2^52 rounds to a whole number and leaves
-// it in the low word), so the rounding to 32 happens to an angle of at most an eighth of a turn, where the series of sin and cos need
-// five terms each: the first term left out is below x^11 / 11! = 2e-9.  The quarter is a swap and two signs.
-__device__ __forceinline__ float2 rope_cos_sin(double turns) {
+// cos and sin of p (turn + low) turns.  The product is formed to twice 64 bits and its whole turns come off first, so every position that 64 bits
+// hold keeps its angle (10^12 tokens out, a product rounded to 64 bits is off by 1e-4; past 2^50 it has no fraction).  Then the nearest quarter
+// turn comes off (adding 1.5 2^52 rounds to a whole number and leaves it in the low word), so the one rounding to 32 happens to an angle of at most
+// pi / 4: 2^-25.  There the series of sin and cos need five terms each: the first term left out is below x^11 / 11! = 2e-9.  The quarter is a
+// swap and two signs.
+__device__ __forceinline__ float2 rope_cos_sin(double p, double turn, double low) {
+  double turns = fma(p, low, fma(p, turn, -rint(p * turn)));   // the inner sum is exact to 2^-54 of itself
+  turns -= rint(turns);
   const double big = 6755399441055744.0, t = fma(4.0, turns, big), q = t - big;
   const int k = __double2loint(t);
-  const float x = 6.283185307179586f * (float)fma(-0.25, q, turns), y = x * x;
+  const float x = (float)(6.283185307179586 * fma(-0.25, q, turns)), y = x * x;
   const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 2.755731922e-6f, -1.984126984e-4f), 8.333333333e-3f), -1.666666667e-1f), x);
   const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -2.755731922e-7f, 2.480158730e-5f), -1.388888889e-3f), 4.166666667e-2f), -0.5f), 1.f);
   const float cs = (k & 1) ? s : c, sn = (k & 1) ? c : s;
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
         const int k = i / half, pair = i - k * half;
         float2 v = make_float2(1.f, 0.f);
         if (pair < a.pairs) {
-          v = rope_cos_sin(rope_position(a, tok0 + k, a.axis[pair]) * a.turn[pair]);
+          v = rope_cos_sin(rope_position(a, tok0 + k, a.axis[pair]), a.turn[pair], a.turn_low[pair]);
         }
         cs[i] = v;
       }
@@ -430,11 +435,23 @@ int rope_run(const scgg_rope_args* p, bool bwd, const char* what, void* workspac
     if (bwd) a.flat &= p->g_stride_b[s] == p->g_stride_n[s] * p->N;
   }
   if (p->B > 1 && p->n_sections > 0) a.flat &= p->pos_stride_b == p->pos_stride_n * p->N;
-  for (int i = 0; i < p->n_sections; ++i)
-    for (int j = 0; j < p->sections[i]; ++j) {
-      a.turn[a.pairs] = pow(p->theta, -(double)j / (double)p->sections[i]) * 0.15915494309189533577;   // 1 / (2 pi)
+  for (int i = 0; i < p->n_sections; ++i) {
+    const int n = p->sections[i];
+    if (n == 0) continue;
+    // theta^(-j / n) (1 / (2 pi)) as a sum of two: 1 / (2 pi) is one, the powers have long double's 64 bits less one step for each factor.
+    // theta^(-1 / n): one Newton step on theta r^n = 1 from the 53 bits of pow (powl takes 0.4 us an axis)
+    const double pi2 = 0x1.45f306dc9c883p-3, pi2_low = -0x1.6b01ec5417056p-57, root = pow(p->theta, -1.0 / n);
+    long double power = 1.0L, square = root, f = 1.0L;
+    for (int bit = n; bit > 0; bit >>= 1, square *= square)
+      if (bit & 1) power *= square;
+    const long double ratio = root + root * (1.0L - (long double)p->theta * power) / n;
+    for (int j = 0; j < n; ++j, f *= ratio) {
+      const long double t = f * pi2;                                        // exact for j = 0
+      a.turn[a.pairs] = (double)t;
+      a.turn_low[a.pairs] = (double)(t - a.turn[a.pairs] + f * pi2_low);
       a.axis[a.pairs++] = (uint8_t)i;
     }
+  }
   if (a.pairs == 0 && !(bwd && norm)) plan.lds = 0;
   if (bwd && norm) {
     const size_t need = (size_t)blocks * p->D * sizeof(float);

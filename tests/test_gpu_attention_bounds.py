@@ -115,3 +115,32 @@ def test_rope_over_more_tiles_than_a_launch_has_workgroups():
     want, _ = axial_rope(q[:, :64], None, pos.expand(64, 1), (1,))
     got, _ = axial_rope(q, None, pos.expand(N, 1), (1,))
     assert bool((got.view(torch.int32) == want.view(torch.int32)[0, 0, 0, 0]).all())
+
+
+@pytest.mark.parametrize("kind", ["i64", "f64", "f32"])
+def test_far_whole_positions_keep_their_angle(kind):
+    """Pairs of an angular step of 1 (sections of one pair), where the angle is the position itself: cos and sin of positions up to 2^62, of timestamps, of
+    2^53 - 1.  The angle comes off the position to 2^-25 (its rounding to 32 bits, below pi / 4) and 2^-35 (2^60 turns times the 2^-106 that two terms
+    leave, times 2 pi, and the series' end), cos and sin are formed in a few steps of 2^-24: the 8 u of the rotation."""
+    import math
+    from semantically_consistent_graph_generation_amd.attention import axial_rope
+    at = [3, 10 ** 9 + 7, 10 ** 12 + 1, 2 ** 40 + 1, 2 ** 50 + 3, 2 ** 53 - 1, 1_700_000_000_123_456_768, 2 ** 62, -(2 ** 62) - 2 ** 12, -7, 0]
+    pos = torch.tensor(at, device="cuda")
+    pos = pos if kind == "i64" else pos.to(torch.float64 if kind == "f64" else torch.float32)
+    n = len(at)
+    q = torch.ones(1, n, 1, 4, device="cuda")
+    q[..., 2:] = 0
+    got = axial_rope(q, None, torch.stack((pos, pos.flip(0)), -1), (1, 1))[0].double().cpu()
+    for i in range(n):
+        for pair, x in ((0, float(pos[i])), (1, float(pos[n - 1 - i]))):
+            assert abs(float(got[0, i, 0, pair]) - math.cos(x)) < 8 * 2.0 ** -24 and abs(float(got[0, i, 0, 2 + pair]) - math.sin(x)) < 8 * 2.0 ** -24, (x, pair)
+
+
+def test_positions_past_every_angle_stay_bounded():
+    """Where not even two terms hold the angle (1e25 and beyond) the rotation is some rotation: no length changes."""
+    from semantically_consistent_graph_generation_amd.attention import axial_rope
+    pos = torch.tensor([1e25, -3e30, 3e38], device="cuda")[:, None]
+    q = torch.randn(1, 3, 2, 32, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    got, _ = axial_rope(q, None, pos, (16,), theta=100.0)
+    length = [(t.double()[..., :16] ** 2 + t.double()[..., 16:] ** 2).sqrt() for t in (got, q)]
+    assert float((length[0] - length[1]).abs().max()) < 1e-5
