@@ -276,21 +276,22 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
       }
     __syncthreads();
     for (int d = tid; d < a.D; d += 256) {
-      float v = 0.f;
+      double v = 0.0;
       for (int q = 0; q < groups; ++q) v += red[q * a.D + d];
-      a.partial[(long long)blockIdx.x * a.D + d] = v;
+      a.partial[(long long)blockIdx.x * a.D + d] = (float)v;
     }
   }
 }
 
 // gradient of a weight = sum of its workgroups' partials (rows [0, split) are q's, [split, rows) k's): 16 columns x 64 row lanes per
-// workgroup, lanes added in order
+// workgroup, lanes added in order.  64 bits, as in the sum over a workgroup's groups: the terms cancel to about the root of their number, and some
+// 150 additions of 32 bits in a row would add twice the terms' own rounding
 template <class T>
 __global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ partial, int split, int rows, int D, int w_f32, void* dw0, void* dw1) {
-  __shared__ float red[64][17];
+  __shared__ double red[64][17];
   const int d = blockIdx.x * 16 + (threadIdx.x & 15), rl = threadIdx.x >> 4;
   const int from = blockIdx.y == 0 ? 0 : split, to = blockIdx.y == 0 ? split : rows;
-  float v = 0.f;
+  double v = 0.0;
   if (d < D) {
 #pragma unroll 4
     for (int r = from + rl; r < to; r += 64) v += partial[(long long)r * D + d];
@@ -300,8 +301,8 @@ __global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__
   void* o = blockIdx.y == 0 ? dw0 : dw1;
   if (rl != 0 || d >= D || o == nullptr) return;
   for (int q = 1; q < 64; ++q) v += red[q][threadIdx.x & 15];
-  if (w_f32) static_cast<float*>(o)[d] = v;
-  else static_cast<T*>(o)[d] = (T)v;
+  if (w_f32) static_cast<float*>(o)[d] = (float)v;
+  else static_cast<T*>(o)[d] = (T)(float)v;
 }
 
 template <class T, int V, int CH, bool NORM>
