@@ -170,7 +170,7 @@ class SiT(nn.Module):
         x = x.float().masked_fill(~mask[..., None], 0.0)          # whatever padded rows hold: 0 times a NaN would reach the weights' gradients
         dim = self.hidden_size
         half = self.t_embedder.mlp[0].in_features // 2
-        arg = t.float()[:, None] * torch.exp(torch.arange(half, device=x.device) * (-math.log(10000.0) / half))
+        arg = t.float()[:, None] * torch.exp(torch.arange(half, device=x.device, dtype=torch.float32) * (-math.log(10000.0) / half))
         mlp = self.t_embedder.mlp
         c = F.silu(mlp[2](F.silu(mlp[0](torch.cat((arg.cos(), arg.sin()), -1)))))
         pos, h = x.detach(), self.pos_embedder(x)
@@ -188,7 +188,7 @@ class SiT(nn.Module):
     def _sample_differential(self, x_T, node_mask, steps, noise, seed, graph_id_base):
         """The reference's ancestral chain (cow_diff_nodes_with_3d_checks.py:63-81), one denoiser call and one update per step; the
         draws are those of ``scgg_sit_sample``: Philox normals keyed by (seed, global graph id, node, step), or ``noise``."""
-        beta = torch.linspace(self.beta_start, self.beta_end, self.noise_steps)
+        beta = torch.linspace(self.beta_start, self.beta_end, self.noise_steps, dtype=torch.float32)
         alpha = 1.0 - beta
         alpha_hat = torch.cumprod(alpha, 0)
         mask = node_mask.to(torch.bool)

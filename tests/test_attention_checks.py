@@ -265,3 +265,25 @@ def test_diff_c_entry_refuses_grids_past_the_launch_limit():
         assert L.scgg_diff_attention_forward(C.byref(a), 4096, need, None) != 0 and "one launch" in L.scgg_last_error().decode()
     a = diff_args(**lots, M=4)
     assert L.scgg_diff_attention_backward(C.byref(a), 4096, 1 << 62, None) != 0 and "one launch" in L.scgg_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_sit_differential_runs_in_32_bits_whatever_the_default_type(dtype, monkeypatch):
+    """Network and sampler around the operators (which are replaced by ones that keep shapes): the same bits under another default type."""
+    from semantically_consistent_graph_generation_amd import node_coordinate_diffusion as N
+    monkeypatch.setattr(A, "qk_norm_rope", lambda q, k, *a, **kw: (q, k))
+    monkeypatch.setattr(A, "diff_attention", lambda q, k, v, lam, key_mask: v * lam)
+    torch.manual_seed(5)
+    model = N.SiT(attention="differential", num_transformer_blocks=2, noise_steps=4)
+    x, noise, mask = torch.randn(2, 3, 3), torch.randn(3, 2, 3, 3), torch.ones(2, 3, dtype=torch.bool)
+
+    def run():
+        with torch.no_grad():
+            return model._forward_differential(x, torch.tensor([3, 1]), mask), model.sample(x, mask, noise=noise)
+    want = run()
+    torch.set_default_dtype(dtype)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(want, got))
