@@ -99,6 +99,10 @@ class SiT(nn.Module):
         if differential and (num_heads % 2 or hidden_size % num_heads or (hidden_size // num_heads) % 8 or hidden_size // num_heads > 64):
             raise _lib.ScggError(f"SiT: {num_heads} heads on {hidden_size} channels: differential attention takes an even number of heads "
                                  "of a multiple of 8 up to 64 channels")
+        if differential and not 1 <= in_channels <= attn_ops.MAX_AXES:
+            raise _lib.ScggError(f"SiT: {in_channels} coordinates: differential attention rotates by 1 to {attn_ops.MAX_AXES} axes")
+        if differential and not 0.0 < rope_theta < float("inf"):
+            raise _lib.ScggError(f"SiT: rope_theta has to be positive and finite, got {rope_theta}")
         self.in_channels, self.hidden_size, self.num_heads = in_channels, hidden_size, num_heads
         self.mlp_hidden = int(hidden_size * mlp_ratio)
         self.noise_steps, self.beta_start, self.beta_end = noise_steps, beta_start, beta_end

@@ -287,3 +287,12 @@ def test_sit_differential_runs_in_32_bits_whatever_the_default_type(dtype, monke
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_sit_refuses_what_every_forward_would():
+    from semantically_consistent_graph_generation_amd.node_coordinate_diffusion import SiT
+    for kw in (dict(in_channels=9), dict(in_channels=0), dict(rope_theta=0.0), dict(rope_theta=float("nan"))):
+        with pytest.raises(_lib.ScggError, match="SiT"):
+            SiT(attention="differential", num_transformer_blocks=1, **kw)
+    SiT(attention="differential", num_transformer_blocks=1, in_channels=8)
+    SiT(attention="softmax", num_transformer_blocks=1, in_channels=9)
