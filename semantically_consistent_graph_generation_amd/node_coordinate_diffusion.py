@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import warnings
 
 import torch
 import torch.nn as nn
@@ -161,8 +162,8 @@ class SiT(nn.Module):
 
     def forward(self, x, t, padding_mask):
         """x [B,N,3], t [B] timesteps, padding_mask [B,N] bool -> predicted noise [B,N,3] (valid rows; 0 on padded ones).
-        Differentiable in the parameters and x (through its embedding; the rotation takes it as given) with differential attention,
-        forward only with the reference's."""
+        Differentiable in the parameters with differential attention, forward only with the reference's.  The gradient of x goes through its
+        embedding only: the rotation takes the coordinates as given, so it is not the derivative of the output (a warning says so)."""
         if not x.is_cuda:
             raise _lib.ScggError("SiT.forward runs on the MI355X only; move the inputs to the GPU")
         if self.attention == "differential":
@@ -170,6 +171,8 @@ class SiT(nn.Module):
         return self._forward_engine(x, t, padding_mask)
 
     def _forward_differential(self, x, t, padding_mask):
+        if x.requires_grad and torch.is_grad_enabled():
+            warnings.warn("SiT(attention='differential'): the gradient of x leaves out its part through the rotation by coordinates", stacklevel=3)
         mask = padding_mask.to(torch.bool)
         x = x.float().masked_fill(~mask[..., None], 0.0)          # whatever padded rows hold: 0 times a NaN would reach the weights' gradients
         dim = self.hidden_size

@@ -296,3 +296,19 @@ def test_sit_refuses_what_every_forward_would():
             SiT(attention="differential", num_transformer_blocks=1, **kw)
     SiT(attention="differential", num_transformer_blocks=1, in_channels=8)
     SiT(attention="softmax", num_transformer_blocks=1, in_channels=9)
+
+
+def test_sit_differential_says_that_the_gradient_of_x_is_partial(monkeypatch):
+    import warnings
+    from semantically_consistent_graph_generation_amd import node_coordinate_diffusion as N
+    monkeypatch.setattr(A, "qk_norm_rope", lambda q, k, *a, **kw: (q, k))
+    monkeypatch.setattr(A, "diff_attention", lambda q, k, v, lam, key_mask: v * lam)
+    model = N.SiT(attention="differential", num_transformer_blocks=1)
+    x, t, mask = torch.randn(2, 3, 3), torch.tensor([3, 1]), torch.ones(2, 3, dtype=torch.bool)
+    with pytest.warns(UserWarning, match="rotation"):
+        model._forward_differential(x.clone().requires_grad_(), t, mask)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        model._forward_differential(x, t, mask).sum().backward()
+        with torch.no_grad():
+            model._forward_differential(x.clone().requires_grad_(), t, mask)
