@@ -86,7 +86,8 @@ Args make(const scgg_diff_attention_args* p) {
 // the CUs, few workgroups (of 64).  The split kernel does more work per tile and its join costs by the row, so the more workgroups, the more keys it
 // takes: up to 4 workgroups per tile of keys, and 160.  us a call not split / split, 8 heads, d = 64, dv = 128, bf16: 10 tiles, 32 workgroups 28 / 25, 64
 // 28 / 30; 16 tiles, 64 40 / 34, 96 40 / 47, 120 40 / 52; 32 tiles, 128 73 / 70, 160 68 / 80; 64 tiles, 128 129 / 102, 160 129 / 119, 192 129 / 132;
-// 256 tiles, 160 499 / 343.  One query of 16 heads on 4 x 64 x 2048 keys 253 / 55; 60 queries x 8000 keys 242 / 25.
+// 256 tiles, 160 499 / 343.  One query of 16 heads on 4 x 64 x 2048 keys 253 / 55; 60 queries x 8000 keys 242 / 25.  Causal grids too, though the
+// split kernel walks the tiles that the mask hides: 2 heads of 4096 147 / 102 (fp32 427 / 313), 4 of 2048 78 / 74 (fp32 220 / 186).
 void plan_split(Args& a) {
   const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32);
   const long long others = (long long)a.B * a.H * (((long long)a.N + 63) / 64), most = tiles < 40 ? 4 * tiles : 160;
