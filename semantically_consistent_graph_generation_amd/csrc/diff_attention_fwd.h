@@ -477,9 +477,10 @@ int launch_split(const Args& a, hipStream_t st) {
 // wave / two, bf16, 2048 tokens, d = 64, dv = 128: 288 workgroups 154 / 156, 384 155 / 156, 480 160 / 187, 576 239 / 238, 768 248 / 281 (256 of 4096
 // tokens 212 / 191; d = 32, dv = 64: 384 117 / 96, 480 118 / 129); causal 384 156 / 111, 480 156 / 140, 576 157 / 166, 768 181 / 193.  The bounds are those
 // of the 16-bit types; in fp32 a causal grid gains beyond them too (1024 workgroups 1134 / 991, d = 32 492 / 406, d = 48 844 / 796; 2048 of d = 48 lose,
-// 1559 / 1591).
+// 1559 / 1591).  Up to 64 queries half of the waves would have none: two waves at every number of sequences (bf16, 2048 of 20 tokens, 3 heads of 32 / 64
+// 66 / 55, 512 of 64 tokens, 6 heads 36 / 32, fp32 87 / 64; 700 of 70 tokens, 2 heads 30 / 39, fp32 73 / 78).
 inline bool few_queries(const Args& a) {
-  return (long long)a.B * a.H * (((long long)a.N + 127) / 128) <= (a.causal ? 512 : 384);
+  return a.N <= 64 || (long long)a.B * a.H * (((long long)a.N + 127) / 128) <= (a.causal ? 512 : 384);
 }
 
 template <class T>

@@ -167,3 +167,13 @@ def test_weight_gradients_add_up_without_loss():
             square += float((((got.double() - terms.sum(0)) ** 2) / (terms ** 2).sum(0)).sum())
             count += 32
     assert count == 512 and (square / count) ** 0.5 < 1.5e-7, (square / count) ** 0.5
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("N,causal", [(20, False), (64, True), (65, False)])
+def test_many_short_sequences(N, causal, dtype):
+    """More than 512 workgroups whose queries are 64 at most (two waves share a tile), and just more."""
+    q, k, v, lam, dout, g = make(300, N, N, 2, 2, 32, 64, dtype, N + 9)
+    mask = mask_of("ragged", 300, N, g)
+    check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal),
+          reference(q, k, v, lam, dout, mask, causal, terms=1 if dtype == "fp32" else 2))
