@@ -84,9 +84,9 @@ Args make(const scgg_diff_attention_args* p) {
 
 // Keys split over workgroups (0: not): for up to 32 rows of a key head, and where the queries give the other kernel, one long chain of tiles on a part of
 // the CUs, few workgroups (of 64).  The split kernel does more work per tile and its join costs by the row, so the more workgroups, the more keys it
-// takes: up to 4 workgroups per tile of keys, and 160.  us a call not split / split, 8 heads, d = 64, dv = 128, bf16: 10 tiles, 32 workgroups 28 / 25, 64
-// 28 / 30; 16 tiles, 64 40 / 34, 96 40 / 47, 120 40 / 52; 32 tiles, 128 73 / 70, 160 68 / 80; 64 tiles, 128 129 / 102, 160 129 / 119, 192 129 / 132;
-// 256 tiles, 160 499 / 343.  One query of 16 heads on 4 x 64 x 2048 keys 253 / 55; 60 queries x 8000 keys 242 / 25.  Causal grids too, though the
+// takes: up to 4 workgroups per tile of keys, and 160.  us a call not split / split, 8 heads, d = 64, dv = 128, bf16: 10 tiles, 32 workgroups 28 / 26, 64
+// 28 / 32; 16 tiles, 64 41 / 35, 96 41 / 48, 120 41 / 55; 32 tiles, 128 73 / 72, 160 73 / 82; 64 tiles, 128 139 / 102, 160 139 / 121, 192 139 / 135;
+// 256 tiles, 160 533 / 346.  One query of 16 heads on 4 x 64 x 2048 keys 279 / 55; 60 queries x 8000 keys 260 / 25.  Causal grids too, though the
 // split kernel walks the tiles that the mask hides: 2 heads of 4096 147 / 102 (fp32 427 / 313), 4 of 2048 78 / 74 (fp32 220 / 186).
 void plan_split(Args& a) {
   const long long rows = (long long)a.N * (a.H / a.Hkv), tiles = (a.M + TILE - 1) / TILE, blocks = (long long)a.B * a.Hkv * ((rows + 31) / 32);
@@ -105,7 +105,7 @@ size_t part_bytes(const Args& a) {
 }
 // Queries split over workgroups in the dK / dV kernel: where the keys alone give fewer than two workgroups to each CU, and there are tiles to
 // split.  Each split writes its sums in 32 bits and they are read again, so there are four at most.  Training pass with 1, 2, 4, 8 splits allowed:
-// 4096 causal, 8 heads on 4, 905, 622, 490, 490 us; not causal 1002, 721, 651, 652; 16 heads of 2048 375, 360, 360, 361.
+// 4096 causal, 8 heads on 4, 1053, 711, 551, 550 us; not causal 1172, 838, 756, 756; 16 heads of 2048 433, 413, 412, 414.
 void plan_dkv(Args& a) {
   const long long blocks = (long long)a.B * a.Hkv * ((a.M + 127) / 128), tiles = (long long)((a.N + TILE - 1) / TILE) * (a.H / a.Hkv);
   long long s = blocks > 0 ? 512 / blocks : 1;
@@ -114,10 +114,10 @@ void plan_dkv(Args& a) {
   a.splits = s < 1 ? 1 : (int)s;
 }
 // Keys split over workgroups in the dQ kernel, where the queries (64 to a workgroup) fill about half of the GPU or less.  The splits' dQ and the
-// sweeps' second launch cost about as much as eight tiles.  Training pass, not split / split, 8 heads: 128 workgroups, 16 tiles, fp32, d = 64 418 / 345 us (bf16
-// 162 / 169), 64 tiles, bf16 382 / 300; 160 workgroups, 16 tiles, fp32 436 / 463, 32 tiles 837 / 755 (bf16 225 / 202).  Causal grids of up to two workgroups
+// sweeps' second launch cost about as much as eight tiles.  Training pass, not split / split, 8 heads: 128 workgroups, 16 tiles, fp32, d = 64 417 / 346 us (bf16
+// 177 / 180), 64 tiles, bf16 386 / 297; 160 workgroups, 16 tiles, fp32 440 / 464, 32 tiles 836 / 754 (bf16 256 / 227).  Causal grids of up to two workgroups
 // per CU are split in two: all of them run at once, so the longest is the time, and halving it is worth the join (4096 causal, 8 heads on 4, training pass:
-// 513 -> 490 us).
+// 575 -> 551 us; not causal it would cost 757 -> 780).
 void plan_dq(Args& a) {
   const long long blocks = (long long)a.B * a.H * (((long long)a.N + 63) / 64), tiles = (a.M + TILE - 1) / TILE;
   long long s = blocks == 0 ? 1 : blocks <= (tiles < 32 ? 128 : 160) ? 512 / blocks : a.causal && blocks <= 512 ? 2 : 1;

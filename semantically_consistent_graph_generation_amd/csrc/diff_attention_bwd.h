@@ -6,9 +6,9 @@
 // Two kernels, each of which owns what it writes (no atomics): one over queries for delta and dQ, one over keys for dK and dV.
 // delta comes from a sweep of its own, formed in 32 bits: dlambda is its sum, and dS a difference with it (dO . out would save the sweep, but out
 // is rounded, and the gradient of a row with one key would not be zero).
-// Bound: the vector and the matrix unit.  32 heads of 4096 x 4096, d = 64, dv = 128, bf16, mean of a trace (the forward 643 us): dQ 870 us, vector
-// instructions issue in 57 % of the cycles, the matrix unit is busy in 42; dK 582 us, 47 and 37 %; dV 440 us, 43 and 32 %.  4096 causal, 8 heads on 4:
-// dQ 73 + 97 with 5 + 8 for its joins, dK 116, dV 86, join 12, forward 155.
+// Bound: neither the vector nor the matrix unit alone.  32 heads of 4096 x 4096, d = 64, dv = 128, bf16, mean of a trace (the forward 726 us): dQ 990 us,
+// vector instructions issue in 60 % of the cycles, the matrix unit is busy in 44; dK 730 us, 51 and 39 %; dV 553 us, 45 and 39 %.  4096 causal, 8 heads on 4:
+// dQ 73 + 114 with 5 + 8 for its joins, dK 137, dV 101, join 12, forward 167.
 #pragma once
 #include "diff_attention_fwd.h"
 
@@ -618,8 +618,9 @@ int launch_dkv(const Args& a, hipStream_t st) {
 
 template <class T, int DP, int DVP>
 int launch_bwd(const Args& a, hipStream_t st) {
-  // In 32 bits above d = 32 a wave with all of a tile's keys keeps registers in memory: two share them at every size (2048 workgroups of 128
-  // queries, training pass: d = 64, dv = 128 21.0 -> 15.3 ms, d = 48, dv = 96 13.0 -> 11.1; d = 32 would lose, 5.6 -> 6.2).
+  // In 32 bits above d = 32 a wave with all of a tile's keys keeps many registers in memory: two share them at every size (2048 workgroups of 128
+  // queries, training pass: d = 64, dv = 128 21.0 -> 15.3 ms, d = 48, dv = 96 13.0 -> 11.1; d = 32 would lose, 5.6 -> 6.2).  At d = 64, dv = 128 they
+  // still keep 39 there.
   constexpr bool SHARED = Type<T>::planes == 3 && DP > 32;
   int rc;
   if (a.dq_splits > 1) rc = launch_dq_split<T, DP, DVP>(a, st);

@@ -45,9 +45,9 @@ __device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float 
 // (2 d + 2 d + dv against 2 d + 2 dv per pair of tokens) and half the accumulators, and A, not P1 and P2, is rounded: where the maps
 // cancel, rounding them apart would leave an error of the size of what was cancelled.
 // A workgroup has 4 waves: 4 / KW groups of 32 queries, and KW waves that share a tile's keys.
-// Bound: the vector unit, with the matrix unit behind it: 32 heads of 4096 x 4096, d = 64, dv = 128, bf16, 601 us at best: vector instructions issue in
-// 57 % of the cycles, the matrix unit is busy in 33 %, no LDS bank conflicts (counters).  2 x 8192 queries and keys, ragged, 8 heads, bf16: 1.07 - 1.11 ms,
-// 485 - 503 TFLOP/s of 4 d + 2 dv per pair (a large library matrix product: 1118).
+// Bound: neither unit alone.  32 heads of 4096 x 4096, d = 64, dv = 128, bf16, 622 us: vector instructions issue in 59 % of the cycles, the matrix unit is
+// busy in 40 %, no LDS bank conflicts (counters); a SIMD has two waves, which meet at two barriers a tile.  2 x 8192 queries and keys, ragged, 8 heads,
+// bf16: 1.27 ms, 424 TFLOP/s of 4 d + 2 dv per pair (a large library matrix product: 1118), the second term's products not counted.
 template <class T, int DP, int DVP>
 struct FwdShape {
   static constexpr int P = Type<T>::planes;
