@@ -177,3 +177,53 @@ def test_many_short_sequences(N, causal, dtype):
     mask = mask_of("ragged", 300, N, g)
     check(run_all(q, k, v, lam, dout, key_mask=mask, causal=causal),
           reference(q, k, v, lam, dout, mask, causal, terms=1 if dtype == "fp32" else 2))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("N,M", [(70, 90), (3, 700), (130, 1300)])
+def test_a_sequence_without_keys_may_hold_anything(N, M, dtype):
+    """Whole sequences that the mask leaves nothing of, without `causal`: NaN in all of their rows."""
+    q, k, v, lam, dout, g = make(3, N, M, 2, 1, 32, 64, dtype, N + M + 3)
+    mask = mask_of("random", 3, M, g)
+    mask[1] = False
+    clean = run_all(q, k, v, lam, dout, key_mask=mask)
+    dirty = [t.clone() for t in (q, k, v, dout)]
+    for t in dirty:
+        t[1] = float("nan")
+    for a, b in zip(clean, run_all(*dirty[:3], lam, dirty[3], key_mask=mask)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert not any(t[1].any() for t in clean[:4])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_two_streams_and_graphs_of_the_split_path(dtype):
+    """Few queries against many keys on two streams at once, and as two captured graphs replayed in turn with eager work between."""
+    from semantically_consistent_graph_generation_amd.attention import diff_attention
+    q, k, v, lam, dout, g = make(4, 2, 6000, 4, 2, 64, 128, dtype, 31)
+    q2 = (q * 0.5).contiguous()
+    want, want2 = diff_attention(q, k, v, lam, causal=True), diff_attention(q2, k, v, lam)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(diff_attention(q, k, v, lam, causal=True))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(diff_attention(q2, k, v, lam))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, want) for x in got[0]) and all(torch.equal(x, want2) for x in got[1])
+    graphs, held = [], []
+    for x, causal in ((q, True), (q2, False)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(diff_attention(x, k, v, lam, causal=causal))
+        graphs.append(graph)
+    for _ in range(3):
+        k.mul_(1.01)
+        for graph in graphs:
+            graph.replay()
+        eager = diff_attention(q, k, v, lam, causal=True), diff_attention(q2, k, v, lam)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
