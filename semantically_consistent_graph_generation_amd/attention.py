@@ -14,11 +14,12 @@ and gradients are contiguous and of the inputs' type; statistics, sums and angle
 Calls enqueue on the current stream of the tensors' device, never synchronise, give equal bits for equal inputs, and can be
 captured into a HIP graph.  A tensor that another stream filled needs that stream's work to be waited for first, as with any
 torch operation.  There is no CPU path (``_lib.ScggError``); second derivatives and forward-mode derivatives are not built, and
-``torch.jit.trace`` is refused.
+``torch.jit.trace`` and ``make_fx`` are refused.
 """
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 from torch.autograd import forward_ad
@@ -50,9 +51,15 @@ def _check_heads(what, name, t, like=None):
         _fail(what, f"{name} is {t.dtype} on {t.device}, q is {like.dtype} on {like.device}")
 
 
+try:                                                          # the mode in which make_fx records; None outside of one (0.1 us, get_proxy_mode takes 0.9)
+    _recording = functools.partial(torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY)
+except AttributeError:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode as _recording
+
+
 def _check_mode(what, *ts):
     """The launches are seen by reverse-mode autograd and by stream capture, and by nothing else that records torch's operations."""
-    if torch.jit.is_tracing():
+    if torch.jit.is_tracing() or _recording() is not None:
         _fail(what, "it cannot be traced (the trace would hold the empty outputs and not the kernels)")
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         _fail(what, "forward-mode derivatives are not built")

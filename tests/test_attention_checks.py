@@ -312,3 +312,15 @@ def test_sit_differential_says_that_the_gradient_of_x_is_partial(monkeypatch):
         model._forward_differential(x, t, mask).sum().backward()
         with torch.no_grad():
             model._forward_differential(x.clone().requires_grad_(), t, mask)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_make_fx_is_refused(which, monkeypatch):
+    """The graph would hold the allocation of the output and no kernel, as a trace would."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    monkeypatch.setattr(A, "_check_device", lambda *a: None)
+    monkeypatch.setattr(A, "_call", lambda *a: 0)
+    f, ts = calls()[which]
+    with pytest.raises(_lib.ScggError, match="traced"):
+        make_fx(f)(*ts)
+    f(*ts)
