@@ -563,7 +563,8 @@ size_t scgg_rope_workspace_bytes(const scgg_rope_args* args);
  * heads 2h, 2h + 1 of q, k1, k2 the heads 2g, 2g + 1 of k and v the head g of v, g = h / (H / Hkv).  key_mask[b,j] = 0 hides
  * key j (whatever its k and v hold); causal hides key j from query i where j > i + M - N (its k and v have to be finite, as other
  * queries see it).  A query that sees no key gives a row of zeros, and no gradient (whatever its q and dout hold).  d, dv: multiples of 8, d <= 64, dv <= 128.  Bases and strides of q, k, v and dout: multiples of
- * 16 bytes, and so have the bases of out, stats, dq, dk and dv_out; 64 rows of a tensor (of two heads) have to lie within 2 GiB. */
+ * 16 bytes, and so have the bases of out, stats, dq, dk and dv_out; 64 rows of a tensor (of two heads) have to lie within 2 GiB.
+ * Grids of 2^24 workgroups and more (one for up to 128 queries of a head and sequence at least) are refused. */
 typedef struct scgg_diff_attention_args {
   const void* q;                       /* [B,N,2 H,d] */
   const void* k;                       /* [B,M,2 Hkv,d] */
